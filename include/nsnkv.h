@@ -44,6 +44,7 @@ extern "C" {
 #define NSNKV_ST_OUTPUT_NONFINITE 8  /* NaN/Inf in a reconstruction or attention output */
 #define NSNKV_ST_TIMEOUT 32          /* a bounded wait inside a kernel gave up */
 #define NSNKV_ST_CAPACITY 64         /* an appended token found its tail buffer full (not stored) */
+#define NSNKV_ST_PAGE 128            /* a page, sequence or row number outside its array (skipped) */
 
 /* element dtypes */
 #define NSNKV_F16 0
@@ -477,6 +478,118 @@ int nsnkv_int3asym_decode(const uint8_t *packed, const uint16_t *norm, const uin
 int nsnkv_k1c_scores(int recipe, int64_t batch, int n_q, int n_kv, int64_t tokens, int head_dim, const void *q,
                      const void *code, const uint16_t *k_min, const uint16_t *k_step, const uint16_t *eff_norm,
                      float *scores, void *stream);
+
+/*
+ * Attention over whole prompts packed one after another: sequence s is tokens
+ * [cu_seqlens[s], cu_seqlens[s + 1]) of q, k, v and out, and its row i attends to its tokens
+ * 0 .. i (causal) or to all of them.  What the model's own attention computes over a prompt
+ * before the cache compresses it (the OFFICIAL arm of
+ * experiments/nb06/source/loop_kv_nb06_attention.py:33-88), without padding or repeated heads.
+ *   tokens       rows of q, k, v and out; cu_seqlens int32 [seqs + 1] on the device, ascending,
+ *                within [0, tokens] (values outside are clamped); rows that no sequence covers
+ *                are not written
+ *   longest      the longest sequence as far as the caller knows: it sizes the grid only
+ *   q, k, v      token t of head j starts at element t * tok + j * head of its own strides
+ *                (views of one fused projection are fine); 128 contiguous channels per head,
+ *                strides multiples of 8 elements, pointers 16-byte aligned; dtype F16 or BF16
+ *   out          [tokens][hq][128] of dtype; lse [tokens][hq] natural log-sum-exp of the scaled
+ *                scores (may be NULL)
+ * Scores use scale 1/sqrt(128); softmax statistics and accumulation are fp32, the
+ * probabilities are rounded to dtype for the product with V.  A token that a row does not
+ * see does not reach it, NaN and infinities included.  NSNKV_ST_OUTPUT_NONFINITE when an
+ * output is not finite.
+ */
+int nsnkv_prompt_attn(int64_t tokens, int32_t seqs, int64_t longest, int hq, int h, int dtype, int causal,
+                      const void *q, int64_t q_tok, int64_t q_head, const void *k, int64_t k_tok, int64_t k_head,
+                      const void *v, int64_t v_tok, int64_t v_head, const int32_t *cu_seqlens, void *out, float *lse,
+                      int32_t *status, void *stream);
+
+/*
+ * Attention of many query rows over a sealed prefix that they share, computed once for all:
+ * each block record of the prefix is read and restored once per kv head and row tile, K and V
+ * rounded to dtype as restore_group(g, dtype) rounds them (loop_kv_nb06_codec.py:36-38), and
+ * the result is merged with each row's attention over its own tokens.  No counterpart in the
+ * reference.
+ *   q            [rows][hq][128] of dtype (rows: one per sequence when decoding, any number
+ *                of new tokens otherwise); every row sees its group's whole prefix
+ *   records      block records (INT3 or INT5, codes in the records' orders): record of kv head
+ *                j, page p at j * rec_stride_head + p * rec_stride_page bytes, p < pages
+ *   table        int32 [groups][table_stride]: group g's prefix is its first n_pages[g]
+ *                entries (n_pages NULL: max_pages of them)
+ *   row_offsets  int32 [groups + 1]: group g's rows are positions row_offsets[g] ..
+ *                row_offsets[g + 1] - 1 (NULL: one group of all rows); row_index int32 [rows]:
+ *                the query row at each position (NULL: the position itself).  Rows outside
+ *                every group have no prefix.
+ *   max_rows     the most rows in a group as far as the caller knows (0: rows); sizes the grid
+ *   o_part, lse_part  fp32 [rows][hq][128] and [rows][hq]: normalised output and natural
+ *                log-sum-exp over each row's own tokens (-inf: none); both NULL: no merge
+ *   out, lse     as for nsnkv_prompt_attn, over prefix and own tokens; a row that sees
+ *                nothing gets zeros and -inf
+ *   workspace    nsnkv_prefix_attn_workspace_bytes() bytes, 16-byte aligned, any contents;
+ *                calls that may run at the same time need separate ones
+ * Status: NSNKV_ST_INPUT_NONFINITE (q or a record's metadata), NSNKV_ST_OUTPUT_NONFINITE,
+ * NSNKV_ST_PAGE (a table entry outside [0, pages): page 0 is read instead), NSNKV_ST_TIMEOUT.
+ */
+int64_t nsnkv_prefix_attn_workspace_bytes(int64_t rows, int32_t groups, int hq, int h, int32_t max_pages);
+int nsnkv_prefix_attn(int64_t rows, int32_t groups, int64_t max_rows, int hq, int h, int bits, int dtype,
+                      const void *q, const uint8_t *records, int64_t pages, int64_t rec_stride_head,
+                      int64_t rec_stride_page, const int32_t *table, int64_t table_stride, const int32_t *n_pages,
+                      int32_t max_pages, const int32_t *row_offsets, const int32_t *row_index, const float *o_part,
+                      const float *lse_part, void *out, float *lse, void *workspace, int64_t workspace_bytes,
+                      int32_t *status, void *stream);
+
+/*
+ * Page operations of a paged cache whose sequences share pages.  page_refs int32 [pages]
+ * counts, for every page p > 0, the entries of block_table [batch][table_stride] equal to p;
+ * a page is free when its count is 0.  Page 0 is the unassigned page: an entry 0 names no
+ * page, and a block sealed through one is lost, never written out of range.  Entries of a
+ * sequence from n_blocks[b] on are pages reserved for its next blocks.  All arrays are on the
+ * device, everything runs in stream order and nothing is read back; numbers out of range are
+ * skipped and set NSNKV_ST_PAGE.  No counterpart in the reference, whose caches grow by
+ * torch.cat (experiments/nb06/source/loop_kv_nb06_packed.py:36-50).
+ *
+ * nsnkv_fork_sequences: sequence dst[i] becomes a copy of sequence src[i], i < count: it drops
+ * its pages, shares src's sealed pages (reserved ones are not shared), and copies src's
+ * counters and tail rows (16-bit tails, strides in rows of 128 elements).  The dst are
+ * distinct and none of them is a src.
+ * nsnkv_free_sequences: sequences drop their pages and are empty.
+ * nsnkv_reserve_pages: every sequence gets pages for its next `ahead` blocks where its entries
+ * n_blocks[b] .. n_blocks[b] + ahead - 1 name none; in (sequence, entry) order they take the
+ * free pages in ascending order.  NSNKV_ST_CAPACITY when too few are free (the rest stay 0).
+ */
+int nsnkv_fork_sequences(int64_t batch, int h, int64_t pages, int32_t *block_table, int64_t table_stride,
+                         int32_t max_blocks, int32_t *n_blocks, int32_t *tail_len, int32_t *page_refs, void *k_tail,
+                         void *v_tail, int64_t tail_stride_seq, int64_t tail_stride_head, int64_t count,
+                         const int32_t *src, const int32_t *dst, int32_t *status, void *stream);
+int nsnkv_free_sequences(int64_t batch, int64_t pages, int32_t *block_table, int64_t table_stride, int32_t max_blocks,
+                         int32_t *n_blocks, int32_t *tail_len, int32_t *page_refs, int64_t count, const int32_t *seqs,
+                         int32_t *status, void *stream);
+int nsnkv_reserve_pages(int64_t batch, int64_t pages, int32_t *block_table, int64_t table_stride, int32_t max_blocks,
+                        const int32_t *n_blocks, int32_t *page_refs, int32_t ahead, int32_t *status, void *stream);
+
+/*
+ * One array of a page pool: page p of head j is `bytes` bytes at base + j * stride_head +
+ * p * stride_page (all multiples of 16).
+ * nsnkv_copy_pages: page dst[i] of every array and head becomes a copy of page src[i] (no dst
+ * is a src of another pair).
+ * nsnkv_compact_pages: with L live pages (page 0 and those with page_refs > 0) the i-th live
+ * page at or above L moves to the i-th free page below L, both in ascending order; table_out
+ * and refs_out get the table and the counts of the moved pages (each may be its input) and
+ * *live (device) gets L.  Freed pages keep their bytes.  workspace:
+ * nsnkv_compact_pages_workspace_bytes(pages) bytes, 4-byte aligned, any contents.
+ */
+#define NSNKV_MAX_PAGE_ARRAYS 8
+typedef struct nsnkv_page_array {
+  void *base;
+  int64_t bytes, stride_head, stride_page;
+} nsnkv_page_array;
+int nsnkv_copy_pages(int h, int64_t pages, int arrays, const nsnkv_page_array *arr, int64_t count, const int32_t *src,
+                     const int32_t *dst, int32_t *status, void *stream);
+int64_t nsnkv_compact_pages_workspace_bytes(int64_t pages);
+int nsnkv_compact_pages(int h, int64_t pages, int arrays, const nsnkv_page_array *arr, int64_t batch,
+                        int32_t max_blocks, const int32_t *block_table, int64_t table_stride, int32_t *table_out,
+                        int64_t table_out_stride, const int32_t *page_refs, int32_t *refs_out, int32_t *live,
+                        void *workspace, int64_t workspace_bytes, int32_t *status, void *stream);
 
 #ifdef __cplusplus
 }

@@ -28,6 +28,7 @@ ST_META_UNDERFLOW = 4
 ST_OUTPUT_NONFINITE = 8
 ST_TIMEOUT = 32
 ST_CAPACITY = 64
+ST_PAGE = 128
 
 ATTN_RECORD_ORDER = 1  # nsnkv_decode_attn_alpha flags
 ATTN_EXACT = 2
@@ -92,6 +93,19 @@ SIGNATURES = [
     ("nsnkv_int3asym_scratch_bytes", c_int64, [c_int64, c_int64, c_int]),
     ("nsnkv_int3asym_encode", c_int, [P, c_int, c_int64, c_int64, c_int, c_int, P, P, P, P, P, c_int64, P, P]),
     ("nsnkv_int3asym_decode", c_int, [P, P, P, P, c_int64, c_int64, c_int, P, P]),
+    ("nsnkv_prompt_attn", c_int, [c_int64, c_int32, c_int64, c_int, c_int, c_int, c_int, P, c_int64, c_int64,
+                                  P, c_int64, c_int64, P, c_int64, c_int64, P, P, P, P, P]),
+    ("nsnkv_prefix_attn_workspace_bytes", c_int64, [c_int64, c_int32, c_int, c_int, c_int32]),
+    ("nsnkv_prefix_attn", c_int, [c_int64, c_int32, c_int64, c_int, c_int, c_int, c_int, P, P, c_int64, c_int64,
+                                  c_int64, P, c_int64, P, c_int32, P, P, P, P, P, P, P, c_int64, P, P]),
+    ("nsnkv_fork_sequences", c_int, [c_int64, c_int, c_int64, P, c_int64, c_int32, P, P, P, P, P, c_int64, c_int64,
+                                     c_int64, P, P, P, P]),
+    ("nsnkv_free_sequences", c_int, [c_int64, c_int64, P, c_int64, c_int32, P, P, P, c_int64, P, P, P]),
+    ("nsnkv_reserve_pages", c_int, [c_int64, c_int64, P, c_int64, c_int32, P, P, c_int32, P, P]),
+    ("nsnkv_copy_pages", c_int, [c_int, c_int64, c_int, P, c_int64, P, P, P, P]),
+    ("nsnkv_compact_pages_workspace_bytes", c_int64, [c_int64]),
+    ("nsnkv_compact_pages", c_int, [c_int, c_int64, c_int, P, c_int64, c_int32, P, c_int64, P, c_int64, P, P, P, P,
+                                    c_int64, P, P]),
     ("nsnkv_k1c_scores", c_int, [c_int, c_int64, c_int, c_int, c_int64, c_int, P, P, P, P, P, P, P]),
 ]
 
@@ -110,6 +124,11 @@ class PagedDesc(ctypes.Structure):
                 ("tail_stride_seq", c_int64), ("tail_stride_head", c_int64),
                 ("seq_counters", P), ("workspace", P), ("workspace_bytes", c_int64), ("status", P),
                 ("host_n_blocks", P), ("host_tail_len", P)]
+
+
+class PageArray(ctypes.Structure):
+    """nsnkv_page_array (include/nsnkv.h), field for field."""
+    _fields_ = [("base", P), ("bytes", c_int64), ("stride_head", c_int64), ("stride_page", c_int64)]
 
 
 _lib = None

@@ -17,8 +17,9 @@ PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libnsnkv.so"
-SOURCES = ["codec.cu", "attention.cu", "int3asym.cu", "scores.cu", "paged_step.cu", "model.cu", "peer_merge.cu"]
-HEADERS = ["nsnkv_common.cuh"]
+SOURCES = ["codec.cu", "attention.cu", "int3asym.cu", "scores.cu", "paged_step.cu", "model.cu", "peer_merge.cu",
+           "prompt.cu", "prefix.cu", "pages.cu"]
+HEADERS = ["nsnkv_common.cuh", "flash_mma.cuh", "record_rows.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -146,3 +146,48 @@ def test_layer_op_argument_errors():
     assert lib.nsnkv_gemv_rows(4, 512, 256, _lib.F16, f, f, f, 2, None) == _lib.ERR_ARG  # unknown flag
     assert lib.nsnkv_gemv_rows(4, 512, 256, _lib.F16, P(8), f, f, fw, None) == _lib.ERR_ARG  # misaligned x
     assert lib.nsnkv_gemv_rows(0, 512, 256, _lib.F16, f, f, f, fw, None) == _lib.OK  # nothing to do
+
+
+def test_shared_prompt_operators_refuse_on_the_host():
+    """Argument errors of the prompt, prefix and page entry points, and calls without work."""
+    from nsn_b200 import _lib
+    lib = _lib.load()
+    P, N = ctypes.c_void_p(16), ctypes.c_void_p(None)
+
+    def prompt(tokens=4, seqs=1, hq=4, h=2, dtype=0, q=P, stride=512, cu=P):
+        return lib.nsnkv_prompt_attn(tokens, seqs, 4, hq, h, dtype, 1, q, stride, 128, P, 256, 128, P, 256, 128, cu, P,
+                                     P, N, N)
+    assert prompt(tokens=0) == _lib.OK and prompt(seqs=0) == _lib.OK
+    for bad in (dict(hq=3), dict(h=0), dict(dtype=2), dict(q=N), dict(q=ctypes.c_void_p(8)), dict(stride=4),
+                dict(cu=N), dict(tokens=-1)):
+        assert prompt(**bad) == _lib.ERR_ARG, bad
+
+    need = lib.nsnkv_prefix_attn_workspace_bytes(4, 1, 8, 2, 10)
+    assert need > 0 and lib.nsnkv_prefix_attn_workspace_bytes(4, 1, 7, 2, 10) == 0
+
+    def prefix(rows=4, groups=1, hq=8, bits=3, dtype=0, pages=20, stride=7680, table_stride=10, offsets=P, part=N,
+               ws=need):
+        return lib.nsnkv_prefix_attn(rows, groups, 4, hq, 2, bits, dtype, P, P, pages, stride * 20, stride, P,
+                                     table_stride, P, 10, offsets, N, part, N, P, P, P, ws, N, N)
+    assert prefix(rows=0) == _lib.OK
+    for bad in (dict(hq=7), dict(bits=4), dict(dtype=2), dict(pages=0), dict(stride=7664), dict(table_stride=9),
+                dict(groups=2, offsets=N), dict(part=P), dict(ws=need - 1)):
+        assert prefix(**bad) == _lib.ERR_ARG, bad
+
+    def fork(batch=2, h=2, pages=8, stride=4, count=1, table=P, tail=P):
+        return lib.nsnkv_fork_sequences(batch, h, pages, table, stride, 4, P, P, P, tail, P, 128, 64, count, P, P, N, N)
+    assert fork(count=0) == _lib.OK
+    for bad in (dict(batch=0), dict(h=0), dict(pages=0), dict(stride=3), dict(table=N), dict(tail=ctypes.c_void_p(8))):
+        assert fork(**bad) == _lib.ERR_ARG, bad
+    assert lib.nsnkv_free_sequences(2, 8, P, 4, 4, P, P, P, 0, N, N, N) == _lib.OK
+    assert lib.nsnkv_free_sequences(2, 8, P, 3, 4, P, P, P, 1, P, N, N) == _lib.ERR_ARG
+    assert lib.nsnkv_reserve_pages(2, 8, P, 4, 4, P, N, 1, N, N) == _lib.ERR_ARG
+    arr = (_lib.PageArray * 1)()
+    arr[0].base, arr[0].bytes, arr[0].stride_head, arr[0].stride_page = 16, 64, 640, 64
+    assert lib.nsnkv_copy_pages(2, 8, 1, arr, 0, N, N, N, N) == _lib.OK
+    assert lib.nsnkv_copy_pages(2, 8, 9, arr, 1, P, P, N, N) == _lib.ERR_ARG
+    arr[0].bytes = 60
+    assert lib.nsnkv_copy_pages(2, 8, 1, arr, 1, P, P, N, N) == _lib.ERR_ARG
+    arr[0].bytes = 64
+    assert lib.nsnkv_compact_pages_workspace_bytes(8) == 100
+    assert lib.nsnkv_compact_pages(2, 8, 1, arr, 2, 4, P, 4, P, 4, P, P, P, P, 99, N, N) == _lib.ERR_ARG

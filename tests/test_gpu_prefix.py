@@ -1,0 +1,229 @@
+"""Shared-prefix attention against its definition in 64 bits over real block records: code
+widths, types, groups, row orders, merges, empty prefixes, statuses and refusals."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+
+
+def pool(h, pages, bits, seed=0):
+    """Block records of `pages` pages encoded by the library from K / V rows of a model's kind."""
+    from nsn_b200 import paged, primitives as w
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    rec, kp, vp = paged.block_record_pools(h, pages, bits, "cuda")
+    for p, boost in ((kp, True), (vp, False)):
+        x = torch.randn((h, pages, 64, 128), generator=g, device="cuda") * torch.exp(
+            0.5 * torch.randn((h, pages, 64, 1), generator=g, device="cuda"))
+        if boost:
+            x[..., [3, 37, 71, 105]] *= 8
+        w.encode_blocks(x.half(), bits, out=p, out_row_stride=pages, out_offset=0, check=False)
+    return rec, kp, vp
+
+
+def rows_of(p, bits, dtype):
+    """Restored rows [h, pages, 64, 128] in dtype: alpha * (min + scale * code), rounded in fp32."""
+    from nsn_b200 import primitives as w
+    h, pages = p["codes"].shape[:2]
+    raw = w.from_code_order(p["codes"].contiguous(), bits, p["code_order"]).reshape(h, pages, -1)
+    stream = ((raw[..., None].int() >> torch.arange(8, device="cuda")) & 1).reshape(h, pages, 64, 128, bits)
+    codes = (stream << torch.arange(bits, device="cuda")).sum(-1).double()
+    d = (p["min"].double()[:, :, None] + p["scale"].double()[:, :, None] * codes).float()
+    return (d * p["alpha"][..., None]).to(dtype)
+
+
+def reference(q, k, v, table, counts, offsets, index, o_part, lse_part):
+    """out, lse and their error bounds (see tests/test_gpu_prompt.py) in 64 bits."""
+    rows, hq = q.shape[:2]
+    h, u = k.shape[0], U[q.dtype]
+    out = torch.zeros(q.shape, dtype=torch.float64, device="cuda")
+    lse = torch.full((rows, hq), -math.inf, dtype=torch.float64, device="cuda")
+    tol, ltol = torch.zeros_like(out), torch.zeros_like(lse)
+    groups = {r: g for g in range(len(counts)) for r in index[offsets[g]:offsets[g + 1]]}
+    for r in range(rows):
+        pages = table[groups[r]][:counts[groups[r]]] if r in groups else []
+        n = 64 * len(pages)
+        for j in range(hq):
+            kv = j // (hq // h)
+            kk = k[kv, pages].reshape(n, 128).double() if n else torch.zeros((0, 128), device="cuda").double()
+            vv = v[kv, pages].reshape(n, 128).double() if n else kk
+            x = kk @ q[r, j].double() / math.sqrt(128)
+            dx = 2.0 ** -20 * (1 + float((kk.abs() @ q[r, j].double().abs()).max() / math.sqrt(128) if n else 0))
+            rest = o_part[r, j].double() if o_part is not None else torch.zeros(128, device="cuda").double()
+            e = lse_part[r, j].double() if lse_part is not None else torch.tensor(-math.inf, device="cuda").double()
+            both = torch.logaddexp(torch.logsumexp(x, 0), e) if n else e
+            if both == -math.inf:
+                continue
+            p, b = torch.exp(x - both), torch.exp(e - both)
+            o, big = p @ vv + b * rest, p @ vv.abs() + b * rest.abs()
+            out[r, j], lse[r, j] = o, both
+            tol[r, j] = u * (o.abs() + big) * 1.01 + (2 * dx + 2.0 ** -20) * big
+            if n:
+                tol[r, j] += n * 2.0 ** -25 * vv.abs().amax()
+            ltol[r, j] = dx + 2.0 ** -21 * (both.abs() + 1)
+    return out, lse, tol, ltol
+
+
+def check(got, ref):
+    (out, lse), (o, e, tol, ltol) = got, ref
+    d = (out.double() - o).abs()
+    assert bool((d <= tol).all()), f"out off by {float((d - tol).max())} over its bound"
+    same = (lse.double() == e) | ((lse.double() - e).abs() <= ltol)
+    assert bool(same.all()), f"lse off by {float((lse.double() - e).abs().nan_to_num().max())}"
+
+
+def case(h, G, bits, dtype, counts, per_group, seed=0, part=True, spare=2, loose=0):
+    g = torch.Generator(device="cuda").manual_seed(seed + 1)
+    pages = sum(counts) + spare
+    rec, kp, vp = pool(h, pages, bits, seed)
+    order = torch.randperm(pages, generator=g, device="cuda").tolist()
+    table, at = [], 0
+    for n in counts:
+        table.append(order[at:at + n])
+        at += n
+    rows = sum(per_group) + loose
+    index = torch.randperm(rows, generator=g, device="cuda").tolist()
+    offsets = [sum(per_group[:i]) for i in range(len(per_group) + 1)]
+    hq = h * G
+    q = torch.randn((rows, hq, 128), generator=g, device="cuda").to(dtype)
+    o_part = lse_part = None
+    if part:
+        o_part = torch.randn((rows, hq, 128), generator=g, device="cuda")
+        lse_part = 5 + torch.randn((rows, hq), generator=g, device="cuda")
+        o_part[0], lse_part[0] = 0, -math.inf
+    wide = max(counts + [1])
+    t = torch.tensor([r + [0] * (wide - len(r)) for r in table], dtype=torch.int32, device="cuda").reshape(-1, wide)
+    dev = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    args = dict(bits=bits, row_offsets=dev(offsets), row_index=dev(index), max_rows=max(per_group), o_part=o_part,
+                lse_part=lse_part)
+    ref = reference(q, rows_of(kp, bits, dtype), rows_of(vp, bits, dtype), table, counts, offsets, index, o_part,
+                    lse_part)
+    return (q, rec, t, dev(counts)), args, ref
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("bits", [3, 5])
+@pytest.mark.parametrize("h,G,counts,per_group", [
+    (2, 4, [1], [1]), (1, 1, [3], [1]), (2, 2, [5], [70]), (3, 3, [2], [17]), (2, 8, [9], [9]), (1, 4, [33], [40]),
+    (2, 4, [4, 1, 7], [3, 9, 1]), (2, 4, [0, 3], [4, 4]), (1, 6, [2, 2], [1, 60]), (8, 4, [20], [2]),
+    (2, 1, [130], [2]), (1, 16, [6], [20])])
+def test_groups_and_lengths(h, G, counts, per_group, bits, dtype):
+    from nsn_b200.prefix import prefix_attention
+    a, kw, ref = case(h, G, bits, dtype, counts, per_group)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    check(prefix_attention(*a, status=status, **kw), ref)
+    assert int(status) == 0
+
+
+@pytest.mark.parametrize("rows", [31, 32, 33, 63, 64, 65, 127, 129, 200])
+def test_row_tiles(rows):
+    """Row counts around the kernels' tile sizes."""
+    from nsn_b200.prefix import prefix_attention
+    a, kw, ref = case(1, 4, 3, torch.float16, [3], [rows], seed=rows)
+    check(prefix_attention(*a, **kw), ref)
+
+
+def test_rows_outside_every_group_and_no_partial():
+    from nsn_b200.prefix import prefix_attention
+    a, kw, ref = case(2, 4, 3, torch.float16, [3, 2], [2, 3], loose=4)
+    check(prefix_attention(*a, **kw), ref)
+    a, kw, ref = case(2, 4, 3, torch.float16, [0, 2], [2, 3], part=False, loose=2)
+    out, lse = prefix_attention(*a, **kw)
+    check((out, lse), ref)
+    assert bool((lse == -math.inf).sum() == 4 * 8) and bool((out[lse == -math.inf] == 0).all())
+
+
+def test_plain_arguments_are_one_group_in_order():
+    from nsn_b200.prefix import prefix_attention
+    (q, rec, t, n), kw, _ = case(2, 4, 3, torch.float16, [6], [10], part=False)
+    kw["row_index"] = None
+    a = prefix_attention(q, rec, t, n, **kw)
+    b = prefix_attention(q, rec, t[0], bits=3)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_strided_records_and_wider_table():
+    """A pool inside a larger one, and a table with more columns than pages in use."""
+    from nsn_b200.prefix import prefix_attention
+    (q, rec, t, n), kw, ref = case(2, 2, 3, torch.float16, [4], [5])
+    big = torch.zeros((3, rec.shape[1] + 9, rec.shape[2] + 256), dtype=torch.uint8, device="cuda")
+    big[:2, 4:4 + rec.shape[1], :rec.shape[2]] = rec
+    wide = torch.full((1, 50), 10 ** 9, dtype=torch.int32, device="cuda")
+    wide[:, :4] = t
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    check(prefix_attention(q, big[:2, 4:4 + rec.shape[1], :rec.shape[2]], wide, n, status=status, **kw), ref)
+    assert int(status) == 0
+
+
+@pytest.mark.parametrize("bits", [3, 5])
+def test_agrees_with_the_bridge_rounding_cache(bits):
+    """One sequence, whole context in the prefix: the paged cache's restore-kernel attention."""
+    from nsn_b200.paged import PagedKVCache
+    from nsn_b200.prefix import prefix_attention
+    g = torch.Generator(device="cuda").manual_seed(3)
+    k, v = (torch.randn((2, 64 * 7, 128), generator=g, device="cuda").half() for _ in range(2))
+    q = torch.randn((1, 8, 128), generator=g, device="cuda").half()
+    kv = PagedKVCache(1, 2, 8, bits=bits, hq=8, restore_rounding="kv")
+    rec = PagedKVCache(1, 2, 8, bits=bits, hq=8)
+    for c in (kv, rec):
+        c.prefill(0, k, v)
+    want = kv.attend(q).double()
+    out, _ = prefix_attention(q, rec.records, rec.block_table[:, :7], bits=bits)
+    # both round K, V, p-free: two fp16 roundings of the output plus p's rounding here
+    assert float((out.double() - want).abs().max()) <= 3 * 2.0 ** -11 * float(want.abs().max()) + 2.0 ** -11
+
+
+def test_statuses():
+    from nsn_b200.prefix import prefix_attention
+    for what, bit in (("page", 128), ("meta", 1), ("q", 1)):
+        (q, rec, t, n), kw, _ = case(1, 2, 3, torch.float16, [3], [4])
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        if what == "page":
+            t[0, 1] = rec.shape[1]
+        if what == "meta":
+            rec[0, int(t[0, 2]), 3072:3074] = 255  # a channel's min: NaN
+        if what == "q":
+            q[1, 0, 5] = math.inf
+        prefix_attention(q, rec, t, n, status=status, **kw)
+        assert int(status) & bit
+
+
+def test_same_result_twice_on_streams_and_in_a_graph():
+    from nsn_b200.prefix import prefix_attention
+    a, kw, ref = case(2, 4, 3, torch.bfloat16, [40], [33])
+    one = prefix_attention(*a, **kw)
+    check(one, ref)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        two = prefix_attention(*a, **kw)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(one[0], two[0]) and torch.equal(one[1], two[1])
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        prefix_attention(*a, out=one[0], lse=one[1], **kw)
+    one[0].zero_()
+    graph.replay()
+    assert torch.equal(one[0], two[0])
+
+
+def test_refusals():
+    from nsn_b200 import ContractError
+    from nsn_b200._lib import NativeError
+    from nsn_b200.prefix import prefix_attention
+    (q, rec, t, n), kw, _ = case(2, 2, 3, torch.float16, [2], [3])
+    bads = [dict(q=q.float()), dict(q=q[:, :3].contiguous()), dict(rec=rec[..., :-16]), dict(t=t.long()),
+            dict(n=n.long()), dict(bits=4), dict(bits=5), dict(row_index=kw["row_index"][:2]),
+            dict(row_offsets=kw["row_offsets"][:1]), dict(lse_part=None), dict(o_part=kw["o_part"].half()),
+            dict(q=q.cpu()), dict(t=torch.cat([t, t]), row_offsets=None)]
+    for bad in bads:
+        a = dict(q=q, rec=rec, t=t, n=n) | {k: x for k, x in bad.items() if k in ("q", "rec", "t", "n")}
+        b = kw | {k: x for k, x in bad.items() if k not in ("q", "rec", "t", "n")}
+        with pytest.raises(ContractError):
+            prefix_attention(a["q"], a["rec"], a["t"], a["n"], **b)
+    with pytest.raises(NativeError):
+        prefix_attention(q, rec, t, n, ws=torch.empty(16, dtype=torch.uint8, device="cuda"), **kw)
