@@ -43,6 +43,7 @@ __host__ __device__ __forceinline__ T *blk_ptr(T *base, int64_t i, int64_t bytes
 // ----------------------------------------------------------------- dtype helpers
 template <typename T> struct Elem;
 template <> struct Elem<__half> {
+  static constexpr bool kBf16 = false;
   static __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
   static __device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
   static __device__ __forceinline__ float2 to_f2(uint32_t bits) {
@@ -51,6 +52,7 @@ template <> struct Elem<__half> {
   }
 };
 template <> struct Elem<__nv_bfloat16> {
+  static constexpr bool kBf16 = true;
   static __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
   static __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
   static __device__ __forceinline__ float2 to_f2(uint32_t bits) {

@@ -6,6 +6,7 @@
 // keys and values; this is that attention for a packed batch, without repeated K / V heads
 // and without padding.
 #include "flash_mma.cuh"
+#include "prompt_tc.cuh"
 
 namespace nsnkv {
 namespace {
@@ -144,6 +145,47 @@ int launch_rows(const PromptArgs &a, int64_t longest, cudaStream_t st) {
   return cudaGetLastError() == cudaSuccess ? NSNKV_OK : NSNKV_ERR_LAUNCH;
 }
 
+// Tensor map of x [tokens][heads][128] with element strides: boxes of 64 channels of one
+// head and 128 tokens, 128-byte swizzle.
+bool make_map(CUtensorMap *map, const void *base, int dtype, int64_t tokens, int heads, int64_t tok, int64_t head) {
+  static const auto encode = [] {
+    void *fn = nullptr;
+    cudaDriverEntryPointQueryResult got;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &got) != cudaSuccess ||
+        got != cudaDriverEntryPointSuccess)
+      fn = nullptr;
+    return reinterpret_cast<decltype(&cuTensorMapEncodeTiled)>(fn);
+  }();
+  if (!encode) return false;
+  const cuuint64_t dims[3] = {kDim, static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(tokens)};
+  // the stride of a dimension of one element is never used
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(heads > 1 ? head : kDim) * 2,
+                                 static_cast<cuuint64_t>(tokens > 1 ? tok : kDim) * 2};
+  const cuuint32_t box[3] = {64, 1, ptc::kN}, step[3] = {1, 1, 1};
+  return encode(map, dtype == NSNKV_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                const_cast<void *>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T>
+int launch_tc(const PromptArgs &p, int dtype, int64_t longest, cudaStream_t st) {
+  ptc::Maps maps;
+  if (!make_map(&maps.q, p.q, dtype, p.tokens, p.hq, p.q_tok, p.q_head) ||
+      !make_map(&maps.k, p.k, dtype, p.tokens, p.h, p.kv_tok, p.kv_head) ||
+      !make_map(&maps.v, p.v, dtype, p.tokens, p.h, p.v_tok, p.v_head))
+    return NSNKV_ERR_CUDA;
+  const ptc::Args a{p.cu, p.out, p.lse, p.q, p.k, p.v, p.tokens, p.q_tok, p.q_head, p.kv_tok, p.kv_head, p.v_tok,
+                    p.v_head, p.hq, p.h, p.causal, p.status};
+  auto kern = ptc::prompt_tc_kernel<T>;
+  const int smem = static_cast<int>(sizeof(ptc::Smem)) + 1024;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return NSNKV_ERR_CUDA;
+  const int64_t pairs = (longest + 2 * ptc::kM - 1) / (2 * ptc::kM);
+  kern<<<dim3(p.hq, p.seqs, static_cast<unsigned>(pairs)), ptc::kThreads, smem, st>>>(a, maps);
+  return cudaGetLastError() == cudaSuccess ? NSNKV_OK : NSNKV_ERR_LAUNCH;
+}
+
 }  // namespace
 }  // namespace nsnkv
 
@@ -164,5 +206,8 @@ extern "C" int nsnkv_prompt_attn(int64_t tokens, int32_t seqs, int64_t longest, 
   PromptArgs a{q, k, v, out, lse, cu_seqlens, tokens, q_tok, q_head, k_tok, k_head, v_tok, v_head, seqs, hq, h,
                causal != 0, status};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (longest > tokens) longest = tokens;
+  if (longest >= 256)
+    return dtype == NSNKV_F16 ? launch_tc<__half>(a, dtype, tokens, st) : launch_tc<__nv_bfloat16>(a, dtype, tokens, st);
   return dtype == NSNKV_F16 ? launch_rows<__half>(a, longest, st) : launch_rows<__nv_bfloat16>(a, longest, st);
 }
