@@ -28,6 +28,7 @@ __device__ __forceinline__ void seq_range(const PromptArgs &a, int s, int64_t &b
   end = min(max(static_cast<int64_t>(a.cu[s + 1]), begin), a.tokens);
 }
 
+constexpr int kSms = 148;
 constexpr int kRowsCta = 64;
 struct RowsSmem {
   uint16_t k[2][fm::kTile][fm::kRow];
@@ -169,20 +170,21 @@ bool make_map(CUtensorMap *map, const void *base, int dtype, int64_t tokens, int
 }
 
 template <typename T>
-int launch_tc(const PromptArgs &p, int dtype, int64_t longest, cudaStream_t st) {
+int launch_tc(const PromptArgs &p, int dtype, cudaStream_t st) {
   ptc::Maps maps;
   if (!make_map(&maps.q, p.q, dtype, p.tokens, p.hq, p.q_tok, p.q_head) ||
       !make_map(&maps.k, p.k, dtype, p.tokens, p.h, p.kv_tok, p.kv_head) ||
       !make_map(&maps.v, p.v, dtype, p.tokens, p.h, p.v_tok, p.v_head))
     return NSNKV_ERR_CUDA;
   const ptc::Args a{p.cu, p.out, p.lse, p.q, p.k, p.v, p.tokens, p.q_tok, p.q_head, p.kv_tok, p.kv_head, p.v_tok,
-                    p.v_head, p.hq, p.h, p.causal, p.status};
+                    p.v_head, p.seqs, p.hq, p.h, p.causal, p.status};
   auto kern = ptc::prompt_tc_kernel<T>;
   const int smem = static_cast<int>(sizeof(ptc::Smem)) + 1024;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return NSNKV_ERR_CUDA;
-  const int64_t pairs = (longest + 2 * ptc::kM - 1) / (2 * ptc::kM);
-  kern<<<dim3(p.hq, p.seqs, static_cast<unsigned>(pairs)), ptc::kThreads, smem, st>>>(a, maps);
+  // at most one pair of row tiles per 256 tokens and one more per sequence
+  const int64_t items = (p.tokens / (2 * ptc::kM) + p.seqs) * p.hq;
+  kern<<<static_cast<unsigned>(items < kSms ? items : kSms), ptc::kThreads, smem, st>>>(a, maps);
   return cudaGetLastError() == cudaSuccess ? NSNKV_OK : NSNKV_ERR_LAUNCH;
 }
 
@@ -207,7 +209,8 @@ extern "C" int nsnkv_prompt_attn(int64_t tokens, int32_t seqs, int64_t longest, 
                causal != 0, status};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (longest > tokens) longest = tokens;
-  if (longest >= 256)
-    return dtype == NSNKV_F16 ? launch_tc<__half>(a, dtype, tokens, st) : launch_tc<__nv_bfloat16>(a, dtype, tokens, st);
+  if (tokens > INT32_MAX || (tokens / 256 + seqs) * hq > INT32_MAX) return NSNKV_ERR_TOO_LARGE;
+  if (longest >= 256 && (reinterpret_cast<uintptr_t>(out) & 31) == 0)
+    return dtype == NSNKV_F16 ? launch_tc<__half>(a, dtype, st) : launch_tc<__nv_bfloat16>(a, dtype, st);
   return dtype == NSNKV_F16 ? launch_rows<__half>(a, longest, st) : launch_rows<__nv_bfloat16>(a, longest, st);
 }

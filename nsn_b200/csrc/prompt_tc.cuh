@@ -1,9 +1,14 @@
 // Prompt attention on the tensor cores (tcgen05), for prompts of a few tiles and more.
 //
-// A CTA attends 256 query rows of one head (two 128-row tiles) over 128-token K / V tiles:
+// One CTA per SM takes items of 256 query rows of one head (two 128-row tiles) and attends
+// them over 128-token K / V tiles:
 //   warps 0-3, 4-7   softmax of row tile 0 and 1, one row per thread
 //   warp 8           issues the MMAs, one thread
-//   warp 9           issues the TMA loads: Q once, K and V through a ring of kStages tiles
+//   warp 9           issues the TMA loads: Q per item, K and V through a ring of kStages tiles
+//   warp 10          lays out the items ahead of the others
+// The code that runs once per item or rarely is kept small (rolled loops, calls): the four
+// schedulers of an SM fetch the softmax loop and the issue loops side by side, and what does
+// not fit their instruction caches stalls every warp.
 // TMEM (512 columns): S0 | S1 | O0 | O1.  Per tile and row tile: S = Q.K^T into S; the
 // softmax warps read a row of S into registers, write P = 2^(x - m) in 16 bits over S and the
 // tensor core adds P.V to O, P read from TMEM.  While one row tile is in its softmax the
@@ -25,14 +30,20 @@ constexpr int kStages = 5;
 constexpr int kTileBytes = kN * kDim * 2;
 constexpr int kThreads = 384;
 constexpr float kRaise = 8.f;
+constexpr int kLag = 3, kAhead = 4;
+constexpr int kPoly = 0, kPolyEvery = 4;  // kPoly of kPolyEvery pairs take ex2_poly
+
+constexpr int kItems = 4;  // items laid out ahead
 
 struct Smem {
   uint8_t q[2][kTileBytes];        // each [2 halves of 64 channels][128 rows][128 B swizzled]
   uint8_t kv[kStages][kTileBytes];
-  uint64_t q_full[2], kv_full[kStages], kv_empty[kStages], s_full[2], p_full[2], o_full[2];
+  uint64_t q_full[2], q_empty[2], kv_full[kStages], kv_empty[kStages], s_full[2], p_full[2][2], o_full[2];
+  uint64_t item_full[kItems], item_empty[kItems];
+  int32_t item[kItems][8];
   uint32_t tmem;
   int32_t failed;
-  int32_t redo[2];
+  uint32_t redo[2][32];
 };
 
 struct Args {
@@ -42,7 +53,7 @@ struct Args {
   const void *q, *k, *v;  // for the guarded second pass
   int64_t tokens;
   int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head;
-  int32_t hq, h, causal;
+  int32_t seqs, hq, h, causal;
   int32_t *status;
 };
 
@@ -50,45 +61,73 @@ struct Maps {
   CUtensorMap q, k, v;
 };
 
-// One softmax warpgroup over its row tile.  Returns false when a wait gave up.
+// 2^x of a pair on the FMA pipes: x = n + f with n the nearest integer and |f| <= 1/2, 2^f by a
+// degree-4 minimax polynomial (relative error 2.6e-6, least squares iterated to the equal
+// ripple), n added to the exponent.  x below -126 gives 2^-126.  The special function unit takes
+// 8 cycles per warp for an exponential, 2048 for the two row tiles of a K / V tile: as long as
+// the tile's MMAs, so a part of the exponentials is done here.
+__device__ __forceinline__ float2 ex2_poly(float2 x) {
+  x.x = fmaxf(x.x, -126.f);
+  x.y = fmaxf(x.y, -126.f);
+  const float2 big = make_float2(12582912.f, 12582912.f);  // 1.5 * 2^23: the sum's low bits hold n
+  const float2 t = tc::add2(x, big);
+  const float2 f = tc::fma2(tc::add2(t, make_float2(-12582912.f, -12582912.f)), make_float2(-1.f, -1.f), x);
+  auto c2 = [](float c) { return make_float2(c, c); };
+  float2 p = tc::fma2(c2(0.009570101276040077f), f, c2(0.05591785907745361f));
+  p = tc::fma2(p, f, c2(0.240247443318367f));
+  p = tc::fma2(p, f, c2(0.6931217908859253f));
+  p = tc::fma2(p, f, c2(0.9999992847442627f));
+  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
+                     __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
+}
+
+// One softmax warpgroup over its row tile.  P is announced in two halves of 64 tokens: the P.V
+// MMAs of the first run while the second is computed.
 template <typename T>
-__device__ __forceinline__ bool softmax_tiles(const Args &a, Smem &S, int t, int tiles, int64_t row, int64_t len,
-                                              int64_t row0, uint32_t tmem, float &m_out, float &l_out) {
+__device__ __forceinline__ void softmax_tiles(const Args &a, Smem &S, int t, int tiles, uint32_t done, int row, int len,
+                                              int row0, uint32_t tmem, float &m_out, float &l_out) {
   constexpr float kSc = kScale * fm::kLog2e;
   const uint32_t lane_base = tmem + (static_cast<uint32_t>((threadIdx.x >> 5) & 3) << 21);  // 32 lanes per warp
   const uint32_t s_at = lane_base + 128 * t, o_at = lane_base + 256 + 128 * t;
   float m = -INFINITY;        // the maximum in use, scaled (log2 units)
-  float2 l = make_float2(0.f, 0.f);
-  const int64_t seen = a.causal ? min(row + 1, len) : len;  // tokens this row sees
+  float2 l = make_float2(0.f, 0.f), l2 = l;
+  const int seen = a.causal ? min(row + 1, len) : len;  // tokens this row sees
+  const int whole = a.causal ? row0 + 1 : len;          // tokens every row of the tile sees
   for (int j = 0; j < tiles; ++j) {
-    if (!mbar_wait_bounded(&S.s_full[t], j & 1, a.status)) return false;
+    tc::wait(&S.s_full[t], (done + j) & 1, &S.failed, a.status);
     tc::fence_after();
-    float s[128];
+    // Two rolled passes over halves of 64 tokens (maximum; exponentials), S read from TMEM in
+    // each: half the code of an unrolled tile.
+    float s[64], mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    const int n = seen - j * kN;
+    const bool masked = j * kN + kN > whole;  // some row of the tile does not see all of it
+    auto load = [&](int h) {
+      tc::ld32(s, s_at + 64 * h);
+      tc::ld32(s + 32, s_at + 64 * h + 32);
+      tc::wait_ld();
+      tc::pin32(s);
+      tc::pin32(s + 32);
+      if (masked) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) tc::ld32(s + 32 * i, s_at + 32 * i);
-    tc::wait_ld();
+        for (int i = 0; i < 64; ++i) s[i] = i < n - 64 * h ? s[i] : -INFINITY;
+      }
+    };
+#pragma unroll 1
+    for (int h = 0; h < 2; ++h) {
+      load(h);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) tc::pin32(s + 32 * i);
-    const int64_t t0 = static_cast<int64_t>(j) * kN;
-    if (a.causal ? t0 + kN > row0 + 1 : t0 + kN > len) {  // some row of the tile does not see all of it
-      const int n = static_cast<int>(max(min(seen - t0, int64_t{kN}), int64_t{0}));
+      for (int i = 0; i < 64; i += 8)
 #pragma unroll
-      for (int i = 0; i < 128; ++i) s[i] = i < n ? s[i] : -INFINITY;
+        for (int c = 0; c < 4; ++c) mx[c] = tc::max3(mx[c], s[i + c], s[i + 4 + c]);
     }
-    float mx[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-    for (int i = 4; i < 128; i += 8) {
-#pragma unroll
-      for (int c = 0; c < 4; ++c) mx[c] = i + 4 + c < 128 ? fmaxf(mx[c], fmaxf(s[i + c], s[i + 4 + c])) : fmaxf(mx[c], s[i + c]);
-    }
-    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * kSc;
+    const float top = kSc * fmaxf(tc::max3(mx[0], mx[1], mx[2]), mx[3]);
     const bool raise = top > m + kRaise;
     if (__any_sync(0xffffffffu, raise)) {
       const float m_new = raise ? top : m;
       if (j > 0) {
         // S of this tile was committed after P.V of the tile before, so O is complete
         const float c = m_new == -INFINITY ? 1.f : fm::ex2(m - m_new);
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < 4; ++i) {
           float o[32];
           tc::ld32(o, o_at + 32 * i);
@@ -100,30 +139,41 @@ __device__ __forceinline__ bool softmax_tiles(const Args &a, Smem &S, int t, int
         }
         l.x *= c;
         l.y *= c;
+        l2.x *= c;
+        l2.y *= c;
       }
       m = m_new;
     }
     const float base = m == -INFINITY ? 0.f : m;
     const float2 sc2 = make_float2(kSc, kSc), nb2 = make_float2(-base, -base);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
+#pragma unroll 1
+    for (int h = 0; h < 2; ++h) {
+      load(h);
+      // Pair e's exponentials issue kLag pairs before its sum and conversion, so that the warp
+      // does not wait for the special function unit's latency.
+      float2 *x = reinterpret_cast<float2 *>(s);
       uint32_t p[16];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float2 x = tc::fma2(make_float2(s[32 * i + 2 * e], s[32 * i + 2 * e + 1]), sc2, nb2);
-        const float2 y = make_float2(fm::ex2(x.x), fm::ex2(x.y));
-        l = tc::add2(l, y);
-        p[e] = fm::round_pair<T>(y.x, y.y);
+      for (int e = 0; e < kAhead; ++e) x[e] = tc::fma2(x[e], sc2, nb2);
+#pragma unroll
+      for (int e = 0; e < 32 + kLag; ++e) {
+        if (e + kAhead < 32) x[e + kAhead] = tc::fma2(x[e + kAhead], sc2, nb2);
+        if (e < 32) x[e] = e % kPolyEvery < kPoly ? ex2_poly(x[e]) : make_float2(fm::ex2(x[e].x), fm::ex2(x[e].y));
+        if (e < kLag) continue;
+        const int d = e - kLag;
+        if (d & 1) l2 = tc::add2(l2, x[d]); else l = tc::add2(l, x[d]);
+        p[d & 15] = fm::round_pair<T>(x[d].x, x[d].y);
+        if ((d & 15) == 15) tc::st16(s_at + 32 * h + (d & ~15), p);
       }
-      tc::st16(s_at + 16 * i, p);
+      tc::wait_st();
+      tc::fence_before();
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) tc::mbar_arrive(&S.p_full[t][h]);
     }
-    tc::wait_st();
-    tc::fence_before();
-    tc::mbar_arrive(&S.p_full[t]);
   }
+  l = tc::add2(l, l2);
   m_out = m;
   l_out = l.x + l.y;
-  return true;
 }
 
 // Rows row0 .. row0 + 127 of one head again, with values that a row does not see kept out of
@@ -185,167 +235,354 @@ __device__ __noinline__ void redo_rows(const Args &a, uint8_t *smem, int t, int6
   }
 }
 
+// A position in the K / V ring: stage and the parity of its barriers.
+struct Ring {
+  uint32_t slot, phase;
+  __device__ __forceinline__ void next() {
+    if (++slot == kStages) {
+      slot = 0;
+      phase ^= 1u;
+    }
+  }
+};
+
+// Work items: (row-tile pair of a sequence, head), longest first: pair p of every sequence that
+// has one before pair p - 1, heads innermost, so that the CTAs running together share K and V
+// in L2 and the short items come last.  Warp-collective: lane i holds the pair counts of
+// sequences i, i + 32, ...  Batches of more than 128 sequences keep the sequences' order.
+struct Item {
+  int begin, len, row0, head;  // the sequence's first token and length, the pair's first row
+  int tiles[2];                // K / V tiles of each row tile; tiles[0] = 0 ends the list
+  int pad[2];
+};
+
+struct Schedule {
+  int np[4];
+  uint32_t pairs;
+
+  __device__ __forceinline__ void range(const Args &a, int s, int64_t &begin, int64_t &len) const {
+    begin = min(max(static_cast<int64_t>(a.cu[s]), int64_t{0}), a.tokens);
+    len = min(max(static_cast<int64_t>(a.cu[s + 1]), begin), a.tokens) - begin;
+  }
+  __device__ __forceinline__ int count(const Args &a, int s) const {
+    if (s >= a.seqs) return 0;
+    int64_t begin, len;
+    range(a, s, begin, len);
+    return static_cast<int>((len + 2 * kM - 1) / (2 * kM));
+  }
+  __device__ __forceinline__ void init(const Args &a) {
+    const int lane = threadIdx.x & 31;
+    pairs = 0;
+    if (a.seqs <= 128) {
+      int n = 0;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        np[c] = count(a, lane + 32 * c);
+        n += np[c];
+      }
+      pairs = __reduce_add_sync(0xffffffffu, n);
+    } else {
+      for (int s = 0; s < a.seqs; s += 32) pairs += __reduce_add_sync(0xffffffffu, count(a, s + lane));
+    }
+  }
+  // pairs at level p or above, over all sequences
+  __device__ __forceinline__ int above(int p) const {
+    int n = 0;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) n += max(np[c] - p, 0);
+    return __reduce_add_sync(0xffffffffu, n);
+  }
+  __device__ __forceinline__ bool item(const Args &a, uint32_t k, Item &it) const {
+    const uint32_t g = gridDim.x, c = blockIdx.x, hq = a.hq;
+    const uint32_t rank = static_cast<uint32_t>(k) * g + (k & 1 ? g - 1 - c : c);  // back and forth over the CTAs
+    it.tiles[0] = it.tiles[1] = 0;
+    if (rank >= pairs * hq) return false;
+    const int lane = threadIdx.x & 31;
+    it.head = static_cast<int>(rank % hq);
+    int r = static_cast<int>(rank / hq), seq = 0, pair = 0;
+    if (a.seqs <= 128) {
+      int lo = 0, hi = __reduce_max_sync(0xffffffffu, max(max(np[0], np[1]), max(np[2], np[3])));
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (above(mid) > r) lo = mid; else hi = mid;
+      }
+      r -= above(lo + 1);
+      pair = lo;
+#pragma unroll
+      for (int c4 = 0; c4 < 4; ++c4) {
+        const uint32_t has = __ballot_sync(0xffffffffu, np[c4] > lo);
+        const uint32_t mine = __ballot_sync(0xffffffffu, np[c4] > lo && __popc(has & ((1u << lane) - 1u)) == r);
+        if (mine) seq = 32 * c4 + __ffs(mine) - 1;
+        r -= __popc(has);
+      }
+    } else {
+      for (int s = 0; s < a.seqs; s += 32) {
+        const int n = count(a, s + lane);
+        int up = n;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+          const int x = __shfl_up_sync(0xffffffffu, up, d);
+          if (lane >= d) up += x;
+        }
+        const uint32_t past = __ballot_sync(0xffffffffu, up > r);
+        if (past) {
+          const int at = __ffs(past) - 1;
+          seq = s + at;
+          pair = __shfl_sync(0xffffffffu, n - up, at) + r;
+          break;
+        }
+        r -= __shfl_sync(0xffffffffu, up, 31);
+      }
+    }
+    int64_t begin, len;
+    range(a, seq, begin, len);
+    it.begin = static_cast<int>(begin);
+    it.len = static_cast<int>(len);
+    it.row0 = pair * 2 * kM;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int first = it.row0 + t * kM;
+      const int keys = a.causal ? min(first + kM, it.len) : it.len;
+      it.tiles[t] = first < it.len ? (keys + kN - 1) / kN : 0;
+    }
+    return true;
+  }
+};
+
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 1) prompt_tc_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps maps) {
+__global__ void __launch_bounds__(kThreads, 1)
+    prompt_tc_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps maps) {
   extern __shared__ uint8_t smem_raw[];
   // the swizzle's pattern repeats every 1024 bytes of the shared address
   Smem &S = *reinterpret_cast<Smem *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t{1023});
   const int tid = threadIdx.x, warp = tid >> 5;
-  const int head = blockIdx.x, kvh = head / (a.hq / a.h);
-  const int64_t begin = min(max(static_cast<int64_t>(a.cu[blockIdx.y]), int64_t{0}), a.tokens);
-  const int64_t len = min(max(static_cast<int64_t>(a.cu[blockIdx.y + 1]), begin), a.tokens) - begin;
-  // longest row tiles first: block z counts them down
-  const int64_t pair = static_cast<int64_t>(gridDim.z) - 1 - blockIdx.z;
-  const int64_t row0 = pair * 2 * kM;
-  if (row0 >= len) return;
-  int tiles[2];
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const int64_t first = row0 + t * kM;
-    const int64_t keys = a.causal ? min(first + kM, len) : len;
-    tiles[t] = first < len ? static_cast<int>((keys + kN - 1) / kN) : 0;
-  }
-  const int all = max(tiles[0], tiles[1]);
+  const int group = a.hq / a.h;
 
   if (warp == 8) {
     tc::tmem_alloc(&S.tmem, 512);
   } else if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&S.q_full[i], 1);
+      mbar_init(&S.q_empty[i], 1);
       mbar_init(&S.s_full[i], 1);
-      mbar_init(&S.p_full[i], 128);
+      mbar_init(&S.p_full[i][0], 4);  // one arrival per softmax warp
+      mbar_init(&S.p_full[i][1], 4);
       mbar_init(&S.o_full[i], 1);
-      S.redo[i] = 0;
     }
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&S.kv_full[i], 1);
       mbar_init(&S.kv_empty[i], 1);
     }
+    for (int i = 0; i < kItems; ++i) {
+      mbar_init(&S.item_full[i], 1);
+      mbar_init(&S.item_empty[i], 10);  // the loader, the MMA warp and eight softmax warps
+    }
     S.failed = 0;
     fence_mbar_init();
   }
+  if (warp == 1) S.redo[0][tid & 31] = S.redo[1][tid & 31] = 0;
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
   const uint32_t tmem = S.tmem;
+  // Item k of this CTA, read by a whole warp; false at the end of the list.
+  auto item = [&](uint32_t k, Item &it) {
+    const uint32_t slot = k % kItems;
+    tc::wait(&S.item_full[slot], k / kItems & 1, &S.failed, a.status);
+    const int4 x = reinterpret_cast<const int4 *>(S.item[slot])[0], y = reinterpret_cast<const int4 *>(S.item[slot])[1];
+    it.begin = x.x, it.len = x.y, it.row0 = x.z, it.head = x.w;
+    // the broadcast tells the compiler that the loop bounds are the warp's
+    it.tiles[0] = __shfl_sync(0xffffffffu, y.x, 0), it.tiles[1] = __shfl_sync(0xffffffffu, y.y, 0);
+    if ((tid & 31) == 0) tc::mbar_arrive(&S.item_empty[slot]);
+    return it.tiles[0] > 0 && !*static_cast<volatile int32_t *>(&S.failed);
+  };
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    if (warp == 9 && tc::elect()) {  // ---- TMA loads; ring tile 2 j is K_j, 2 j + 1 is V_j
-      tc::prefetch_map(&maps.q);
-      tc::prefetch_map(&maps.k);
-      tc::prefetch_map(&maps.v);
-      auto load = [&](uint8_t *dst, const CUtensorMap &map, int hd, int64_t tok, uint64_t *bar) {
+    if (warp == 10) {  // ---- items
+      Schedule sch;
+      sch.init(a);
+      Item it;
+      bool more = true;
+      for (uint32_t k = 0; more; ++k) {
+        more = sch.item(a, k, it);
+        tc::wait(&S.item_empty[k % kItems], (k / kItems & 1) ^ 1, &S.failed, a.status);
+        if (*static_cast<volatile int32_t *>(&S.failed)) it.tiles[0] = 0, more = false;
+        if ((tid & 31) == 0) {
+          reinterpret_cast<int4 *>(S.item[k % kItems])[0] = make_int4(it.begin, it.len, it.row0, it.head);
+          reinterpret_cast<int4 *>(S.item[k % kItems])[1] = make_int4(it.tiles[0], it.tiles[1], 0, 0);
+          tc::mbar_arrive(&S.item_full[k % kItems]);
+        }
+        __syncwarp();
+      }
+    } else if (warp == 9) {  // ---- TMA loads; ring tile 2 j is K_j, 2 j + 1 is V_j
+      const bool lead = tc::elect();
+      if (lead) {
+        tc::prefetch_map(&maps.q);
+        tc::prefetch_map(&maps.k);
+        tc::prefetch_map(&maps.v);
+      }
+      auto load = [&](uint8_t *dst, const CUtensorMap *map, int hd, int tok, uint64_t *bar) {
         mbar_expect_tx(bar, kTileBytes);
-        tc::tma_load_3d(dst, &map, 0, hd, static_cast<int>(tok), bar);
-        tc::tma_load_3d(dst + kTileBytes / 2, &map, 64, hd, static_cast<int>(tok), bar);
+        tc::tma_load_3d(dst, map, 0, hd, tok, bar);
+        tc::tma_load_3d(dst + kTileBytes / 2, map, 64, hd, tok, bar);
       };
-      auto ring = [&](int i) {
-        load(S.kv[i % kStages], i & 1 ? maps.v : maps.k, kvh, begin + static_cast<int64_t>(i >> 1) * kN,
-             &S.kv_full[i % kStages]);
-      };
-      load(S.q[0], maps.q, head, begin + row0, &S.q_full[0]);
-      ring(0);
-      if (tiles[1] > 0) load(S.q[1], maps.q, head, begin + row0 + kM, &S.q_full[1]);
-      int i = 1;
-      bool ok = true;
-      for (; i < 2 * all && ok; ++i) {
-        if (i >= kStages) ok = mbar_wait_bounded(&S.kv_empty[i % kStages], (i / kStages - 1) & 1, a.status);
-        if (ok) ring(i);
+      Ring at{0, 1};    // a fresh barrier counts as the phase before: the first round does not wait
+      uint32_t qn = 0;  // bit t: parity of Q loads of row tile t
+      Item it;
+      for (uint32_t k = 0; item(k, it); ++k) {
+        const int kvh = it.head / group, all = max(it.tiles[0], it.tiles[1]);
+        // Q of row tile 0, K_0, Q of row tile 1, V_0, K_1, ...
+        auto queries = [&](int t) {
+          if (it.tiles[t] == 0) return;
+          tc::wait(&S.q_empty[t], (qn >> t & 1) ^ 1, &S.failed, a.status);
+          qn ^= 1u << t;
+          if (lead) load(S.q[t], &maps.q, it.head, it.begin + it.row0 + t * kM, &S.q_full[t]);
+        };
+        queries(0);
+#pragma unroll 1
+        for (int i = 0; i < 2 * all; ++i) {
+          tc::wait(&S.kv_empty[at.slot], at.phase, &S.failed, a.status);
+          if (lead) load(S.kv[at.slot], i & 1 ? &maps.v : &maps.k, kvh, it.begin + (i >> 1) * kN, &S.kv_full[at.slot]);
+          at.next();
+          if (i == 0) queries(1);
+        }
       }
-      if (!ok) {  // give up, but not before the copies in flight have landed
-        --i;
-        for (int x = max(0, i - kStages); x < i; ++x)
-          mbar_wait_bounded(&S.kv_full[x % kStages], (x / kStages) & 1, a.status);
-      }
-    } else if (warp == 8 && tc::elect()) {  // ---- MMA
+      if (*static_cast<volatile int32_t *>(&S.failed))  // a wait gave up: let the copies in flight land
+        for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+    } else if (warp == 8) {  // ---- MMA
+      // Every lane runs the loops and the waits, so that addresses and descriptors stay in uniform
+      // registers; one lane issues.
+      const bool lead = tc::elect();
       constexpr uint32_t kIdS = tc::instr_desc<T>(kM, kN, false), kIdO = tc::instr_desc<T>(kM, kDim, true);
-      auto scores = [&](int t, int slot) {
-        const uint32_t qa = tc::saddr(S.q[t]), ka = tc::saddr(S.kv[slot]);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const uint32_t off = (k >> 2) * (kTileBytes / 2) + (k & 3) * 32;
-          tc::mma_ss(tmem + 128 * t, tc::smem_desc(qa + off, 16, 1024), tc::smem_desc(ka + off, 16, 1024), kIdS, k > 0);
-        }
-        tc::commit(&S.s_full[t]);
-      };
-      auto values = [&](int t, int slot, bool acc) {
-        const uint32_t va = tc::saddr(S.kv[slot]);
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          tc::mma_ts(tmem + 256 + 128 * t, tmem + 128 * t + 8 * k,
-                     tc::smem_desc(va + k * 2048, kTileBytes / 2, 1024), kIdO, acc || k > 0);
-        tc::commit(&S.o_full[t]);
-      };
-      auto ready = [&](int i) { return mbar_wait_bounded(&S.kv_full[i % kStages], (i / kStages) & 1, a.status); };
-      bool ok = ready(0);
-      for (int t = 0; t < 2 && ok; ++t) {
-        if (tiles[t] == 0) continue;
-        ok = mbar_wait_bounded(&S.q_full[t], 0, a.status);
+      // descriptors in 16-byte units: adding to them moves the start address
+      const uint64_t qd = tc::smem_desc(tc::saddr(S.q[0]), 16, 1024), kd = tc::smem_desc(tc::saddr(S.kv[0]), 16, 1024),
+                     vd = tc::smem_desc(tc::saddr(S.kv[0]), kTileBytes / 2, 1024);
+      auto scores = [&](int t, uint32_t slot) {
+        const uint64_t qa = qd + t * (kTileBytes >> 4), ka = kd + slot * (kTileBytes >> 4);
         tc::fence_after();
-        if (ok) scores(t, 0);
-      }
-      tc::commit(&S.kv_empty[0]);
-      for (int j = 0; j < all && ok; ++j) {
-        const int vi = 2 * j + 1, ki = 2 * j + 2;
-        ok = ready(vi);
-        bool have_k = false;
-        for (int t = 0; t < 2 && ok; ++t) {
-          if (j >= tiles[t]) continue;
-          ok = mbar_wait_bounded(&S.p_full[t], j & 1, a.status);
-          if (!ok) break;
-          tc::fence_after();
-          values(t, vi % kStages, j > 0);
-          if (j + 1 < tiles[t]) {
-            if (!have_k) {
-              ok = ready(ki);
-              have_k = true;
-              if (!ok) break;
-            }
-            scores(t, ki % kStages);
+        if (lead) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t off = ((i >> 2) * (kTileBytes / 2) + (i & 3) * 32) >> 4;
+            tc::mma_ss(tmem + 128 * t, qa + off, ka + off, kIdS, i > 0);
           }
+          tc::commit(&S.s_full[t]);
         }
-        tc::commit(&S.kv_empty[vi % kStages]);
-        if (have_k) tc::commit(&S.kv_empty[ki % kStages]);
+      };
+      auto values = [&](int t, int h, uint32_t slot, bool acc) {
+        const uint64_t va = vd + slot * (kTileBytes >> 4) + h * (4 * 2048 >> 4);
+        tc::fence_after();
+        if (lead) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            tc::mma_ts(tmem + 256 + 128 * t, tmem + 128 * t + 32 * h + 8 * i, va + i * (2048 >> 4), kIdO, acc || i > 0);
+        }
+      };
+      auto signal = [&](uint64_t *bar) {
+        if (lead) tc::commit(bar);
+      };
+      auto ready = [&](const Ring &r) { tc::wait(&S.kv_full[r.slot], r.phase, &S.failed, a.status); };
+      Ring at{0, 0};            // the ring position of the next K or V tile
+      uint32_t qn = 0, pn = 0;  // bit t: parity of the next Q tile, P tile of row tile t
+      auto first = [&](int t, int tiles, const Ring &r) {  // S of an item's first tile
+        tc::wait(&S.q_full[t], qn >> t & 1, &S.failed, a.status);
+        qn ^= 1u << t;
+        ready(r);
+        scores(t, r.slot);
+        if (tiles == 1) signal(&S.q_empty[t]);
+      };
+      Item it, next;
+      bool more = item(0, it), ahead = false;
+      for (uint32_t k = 0; more; ++k) {
+        more = item(k + 1, next);
+        const int n0 = it.tiles[0], n1 = it.tiles[1], all = max(n0, n1);
+        if (!ahead) first(0, n0, at);  // row tile 0 of an item is never empty
+        ahead = false;
+        if (n1 > 0) first(1, n1, at);
+        signal(&S.kv_empty[at.slot]);
+        at.next();
+#pragma unroll 1
+        for (int j = 0; j < all; ++j) {  // P.V of tile j, S of tile j + 1
+          Ring kr = at;                  // V_j at `at`, K_{j + 1} (or the next item's K_0) behind it
+          kr.next();
+          ready(at);
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const int n = t ? n1 : n0;
+            if (j < n) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                tc::wait(&S.p_full[t][h], pn >> t & 1, &S.failed, a.status);
+                values(t, h, at.slot, j > 0 || h > 0);
+              }
+              pn ^= 1u << t;
+              if (j + 1 < n) {
+                ready(kr);
+                scores(t, kr.slot);
+                if (j + 2 == n) signal(&S.q_empty[t]);
+              } else {
+                signal(&S.o_full[t]);
+              }
+            } else if (t == 0 && more) {
+              // row tile 0 is done: start it on the next item while row tile 1 finishes
+              first(0, next.tiles[0], kr);
+              ahead = true;
+            }
+          }
+          signal(&S.kv_empty[at.slot]);
+          if (j + 1 < all) {
+            signal(&S.kv_empty[kr.slot]);
+            kr.next();
+          }
+          at = kr;
+        }
+        it = next;
       }
-      if (!ok) S.failed = 1;
     }
     __syncwarp();
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     const int t = warp >> 2;
-    const int64_t first = row0 + t * kM, row = first + (tid & 127);
-    if (tiles[t] > 0) {
+    uint32_t done = 0, taken = 0;  // S tiles and finished O tiles taken so far
+    Item it;
+    for (uint32_t k = 0; item(k, it); ++k) {
+      const int tiles = it.tiles[t];
+      if (tiles == 0) continue;
+      const int first = it.row0 + t * kM, row = first + (tid & 127);
       float m, l;
-      bool ok = softmax_tiles<T>(a, S, t, tiles[t], row, len, first, tmem, m, l);
-      ok = ok && mbar_wait_bounded(&S.o_full[t], (tiles[t] - 1) & 1, a.status);
-      if (ok) {
-        tc::fence_after();
-        const float inv = m == -INFINITY ? 0.f : __fdiv_rn(1.f, l);
-        const uint32_t o_at = tmem + (static_cast<uint32_t>(warp & 3) << 21) + 256 + 128 * t;
-        T *orow = static_cast<T *>(a.out) + ((begin + row) * a.hq + head) * kDim;
-        int bad = 0;
+      softmax_tiles<T>(a, S, t, tiles, done, row, it.len, first, tmem, m, l);
+      done += tiles;
+      tc::wait(&S.o_full[t], taken & 1, &S.failed, a.status);
+      ++taken;
+      tc::fence_after();
+      const float inv = m == -INFINITY ? 0.f : __fdiv_rn(1.f, l);
+      const uint32_t o_at = tmem + (static_cast<uint32_t>(warp & 3) << 21) + 256 + 128 * t;
+      const int64_t at = static_cast<int64_t>(it.begin + row) * a.hq + it.head;
+      T *orow = static_cast<T *>(a.out) + at * kDim;
+      float2 check = make_float2(0.f, 0.f);  // 0 * y summed: NaN when an output is not finite
+#pragma unroll 1
+      for (int i = 0; i < 4; ++i) {
+        float o[32];
+        tc::ld32(o, o_at + 32 * i);
+        tc::wait_ld();
+        tc::pin32(o);
+        uint32_t w[16];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float o[32];
-          tc::ld32(o, o_at + 32 * i);
-          tc::wait_ld();
-          tc::pin32(o);
-          uint32_t w[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            w[e] = fm::round_pair<T>(o[2 * e] * inv, o[2 * e + 1] * inv);
-            const float2 x = Elem<T>::to_f2(w[e]);
-            bad |= !isfinite(x.x) || !isfinite(x.y);
-          }
-          if (row < len)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              reinterpret_cast<uint4 *>(orow)[4 * i + e] = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+        for (int e = 0; e < 16; ++e) {
+          const float2 y = tc::mul2(make_float2(o[2 * e], o[2 * e + 1]), make_float2(inv, inv));
+          check = tc::fma2(y, make_float2(0.f, 0.f), check);
+          w[e] = fm::round_pair<T>(y.x, y.y);
         }
-        if (bad && row < len) S.redo[t] = 1;
-        if (a.lse && row < len)
-          a.lse[(begin + row) * a.hq + head] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * fm::kLn2;
+        if (row < it.len) {
+          tc::store32(orow + 32 * i, w);
+          tc::store32(orow + 32 * i + 16, w + 8);
+        }
+      }
+      tc::fence_before();  // O is read before the next item's first P is announced
+      if (row < it.len) {
+        if (check.x + check.y != 0.f) atomicOr(&S.redo[t][k >> 5 & 31], 1u << (k & 31));
+        if (a.lse) a.lse[at] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * fm::kLn2;
       }
     }
   }
@@ -353,9 +590,19 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_tc_kernel(const __grid_con
   __syncthreads();
   tc::fence_after();
   if (warp == 8) tc::tmem_release(tmem, 512);
-  // Every copy and MMA has finished: the K / V ring is free for the guarded pass.
-  if (warp < 8 && S.redo[warp >> 2] && !S.failed)
-    redo_rows<T>(a, S.kv[2 * (warp >> 2)], warp >> 2, begin, len, row0 + (warp >> 2) * kM, head, kvh);
+  // Items with a non-finite output once more, guarded; every copy and MMA has finished, so the
+  // ring is free.  (Item k of the CTA is bit k mod 1024: one more item than needed may run.)
+  if (warp < 8 && !S.failed) {
+    const int t = warp >> 2;
+    if (__any_sync(0xffffffffu, S.redo[t][tid & 31] != 0)) {
+      Schedule sch;
+      sch.init(a);
+      Item it;
+      for (uint32_t k = 0; sch.item(a, k, it); ++k)
+        if (S.redo[t][k >> 5 & 31] >> (k & 31) & 1 && it.tiles[t] > 0)
+          redo_rows<T>(a, S.kv[2 * t], t, it.begin, it.len, it.row0 + t * kM, it.head, it.head / group);
+    }
+  }
 }
 
 }  // namespace ptc

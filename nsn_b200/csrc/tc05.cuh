@@ -17,6 +17,24 @@ __device__ __forceinline__ uint32_t saddr(const void *p) {
 __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(saddr(bar)) : "memory");
 }
+// Waits of kernels whose warps hand tiles to one another.  A wait polls without sleeping for as
+// long as a tile takes, then with sleeps; one that gives up sets NSNKV_ST_TIMEOUT and *failed
+// (shared memory), and every later wait returns at its first sleep, so the kernel runs to its
+// end over whatever its buffers hold.  Nothing is returned: control flow stays warp-uniform.
+__device__ __noinline__ void wait_long(uint64_t *bar, uint32_t phase, volatile int32_t *failed, int32_t *status) {
+  for (uint32_t i = 0; i < kWaitPolls && !*failed; ++i) {
+    if (mbar_try_wait(bar, phase)) return;
+    __nanosleep(64);
+  }
+  *failed = 1;
+  set_status(status, NSNKV_ST_TIMEOUT);
+}
+__device__ __forceinline__ void wait(uint64_t *bar, uint32_t phase, int32_t *failed, int32_t *status) {
+#pragma unroll 1
+  for (int i = 0; i < 4096; ++i)
+    if (mbar_try_wait(bar, phase)) return;
+  wait_long(bar, phase, failed, status);
+}
 // Completes one arrival on `bar` when every MMA issued so far by this thread has finished.
 __device__ __forceinline__ void commit(uint64_t *bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(saddr(bar))
@@ -142,6 +160,19 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
       : "=l"(d)
       : "l"(*reinterpret_cast<uint64_t *>(&a)), "l"(*reinterpret_cast<uint64_t *>(&b)));
   return *reinterpret_cast<float2 *>(&d);
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// 32 bytes in one store: a whole sector (dst 32-byte aligned).
+__device__ __forceinline__ void store32(void *dst, const uint32_t *w) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
 }
 
 // ----------------------------------------------------------------- TMA
