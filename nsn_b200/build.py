@@ -19,7 +19,7 @@ CSRC = PKG / "csrc"
 LIB = PKG / "libnsnkv.so"
 SOURCES = ["codec.cu", "attention.cu", "int3asym.cu", "scores.cu", "paged_step.cu", "model.cu", "peer_merge.cu",
            "prompt.cu", "prefix.cu", "pages.cu"]
-HEADERS = ["nsnkv_common.cuh", "flash_mma.cuh", "record_rows.cuh", "tc05.cuh", "prompt_tc.cuh"]
+HEADERS = ["nsnkv_common.cuh", "flash_mma.cuh", "record_rows.cuh", "tc05.cuh", "prompt_tc.cuh", "prefix_tc.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -398,7 +398,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
 
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 10) {  // ---- items
       Schedule sch;
       sch.init(a);
@@ -542,7 +541,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     __syncwarp();
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     const int t = warp >> 2;
     uint32_t done = 0, taken = 0;  // S tiles and finished O tiles taken so far
     Item it;

@@ -21,7 +21,7 @@ __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
 // long as a tile takes, then with sleeps; one that gives up sets NSNKV_ST_TIMEOUT and *failed
 // (shared memory), and every later wait returns at its first sleep, so the kernel runs to its
 // end over whatever its buffers hold.  Nothing is returned: control flow stays warp-uniform.
-__device__ __noinline__ void wait_long(uint64_t *bar, uint32_t phase, volatile int32_t *failed, int32_t *status) {
+static __device__ __noinline__ void wait_long(uint64_t *bar, uint32_t phase, volatile int32_t *failed, int32_t *status) {
   for (uint32_t i = 0; i < kWaitPolls && !*failed; ++i) {
     if (mbar_try_wait(bar, phase)) return;
     __nanosleep(64);
@@ -109,6 +109,14 @@ __device__ __forceinline__ void ld32(float *r, uint32_t addr) {
         "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
       : "r"(addr));
 }
+__device__ __forceinline__ void ld16(float *r, uint32_t addr) {
+  uint32_t *u = reinterpret_cast<uint32_t *>(r);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+        "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
+      : "r"(addr));
+}
 __device__ __forceinline__ void st32(uint32_t addr, const uint32_t *u) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
@@ -133,6 +141,12 @@ __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.
 __device__ __forceinline__ void pin32(float *r) {
   asm volatile(""
                : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]), "+f"(r[8]), "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15]), "+f"(r[16]), "+f"(r[17]), "+f"(r[18]), "+f"(r[19]), "+f"(r[20]), "+f"(r[21]), "+f"(r[22]), "+f"(r[23]), "+f"(r[24]), "+f"(r[25]), "+f"(r[26]), "+f"(r[27]), "+f"(r[28]), "+f"(r[29]), "+f"(r[30]), "+f"(r[31])
+               :
+               :);
+}
+__device__ __forceinline__ void pin16(float *r) {
+  asm volatile(""
+               : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]), "+f"(r[8]), "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15])
                :
                :);
 }
