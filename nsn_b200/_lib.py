@@ -171,6 +171,32 @@ def stream_handle(device=None) -> c_void_p:
     return c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+def raw_stream(index: int) -> int:
+    """The current stream of device `index` as an integer handle (no Stream object is made)."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+_scratch: dict = {}
+
+
+def scratch(nbytes: int, device, stream: int) -> torch.Tensor:
+    """Reusable device scratch of at least `nbytes`, one buffer per (device, stream): calls on one
+    stream run in order and may share it, calls on different streams get different ones."""
+    buf = _scratch.get((device.index, stream))
+    if buf is None or buf.numel() < nbytes:
+        buf = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
+        _scratch[(device.index, stream)] = buf
+    return buf
+
+
+def call_on(index: int, fn, *args) -> int:
+    """fn(*args) with device `index` current."""
+    if torch.cuda.current_device() == index:
+        return fn(*args)
+    with torch.cuda.device(index):
+        return fn(*args)
+
+
 def check(rc: int, what: str):
     if rc != OK:
         names = {ERR_ARG: "invalid argument", ERR_LAUNCH: "launch failed", ERR_UNSUPPORTED: "unsupported",

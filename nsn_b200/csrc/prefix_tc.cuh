@@ -6,8 +6,9 @@
 //   warps 8-15       restore: a block's codes become its K and V rows in T, in shared memory
 //   warp 16          issues the MMAs, one thread
 //   warp 17          loads block records (one bulk copy each)
-// TMEM (512 columns): two buffers of S per row tile (64 columns each), O0 | O1.  S of block
-// j + 1 is computed while block j is in its softmax; P overwrites its S buffer.
+// TMEM (512 columns): two buffers of S per softmax team (64 columns each), O0 | O1.  S of the
+// next blocks is computed while a block is in its softmax; P overwrites its S buffer.  With one
+// row tile both softmax teams work on it, on alternate blocks, and join their halves at the end.
 //
 // What bounds it is the restore: 16384 values a block, about four instructions each, whatever
 // the rows.  A code is moved to bits 13..22 of a word and one AND-OR with the bits of 1.0f makes
@@ -27,19 +28,25 @@ namespace xtc {
 
 constexpr int kM = 128;
 constexpr int kThreads = 640;
-constexpr int kStages = 3;
+// A maximum is taken this much (log2 units) above the block's: scores may grow by 2^21 before
+// the next raise, and p of the largest, 2^-6, leaves fp16's 2^-24 far below its rounding.
+constexpr float kHeadroom = 6.f;
+constexpr int kStages = 4;  // restored blocks held
 constexpr int kRowsBytes = kBlock * kDim * 2;  // K or V of one block
 
-template <int BITS> constexpr int kRaw = BITS == 3 ? 4 : 3;  // records in flight
+// Records in flight: their own slots, and with one row tile the slots that fit the other tile's Q.
+template <int BITS> constexpr int kRaw = BITS == 3 ? 3 : 2;
+template <int BITS> constexpr int kRawWide = kRaw<BITS> + kM * kDim * 2 / rr::Rec<BITS>::kBytes;
 
 template <int BITS>
 struct Smem {
   uint8_t q[2][kM * kDim * 2];
   uint8_t kv[kStages][2][kRowsBytes];  // each [2 halves of 64 channels][64 tokens][128 B swizzled]
   uint8_t raw[kRaw<BITS>][rr::Rec<BITS>::kBytes];
-  float2 ab[2][2][kDim];               // [block parity][K, V][channel]: a, b of the channel's codes
-  uint64_t raw_full[kRaw<BITS>], raw_empty[kRaw<BITS>], full[kStages], empty[kStages];
+  float2 ab[2][2][kDim];               // [team][K, V][channel]: a, b of the channel's codes
+  uint64_t raw_full[kRawWide<BITS>], raw_empty[kRawWide<BITS>], full[kStages], empty[kStages];
   uint64_t q_full[2], s_full[2][2], p_full[2][2], o_done[2];
+  float e_other[kM];  // log-sum-exps of the second half of the blocks
   uint32_t tmem;
   int32_t failed;
 };
@@ -67,22 +74,35 @@ __device__ __forceinline__ void windows(const uint32_t (&s)[(BITS + 1) / 2], uin
   }
 }
 
+template <int I> struct Int { static constexpr int value = I; };
+
+// (x & mask) | one: one logic instruction, with the bits of 1.0f in a register.
+template <uint32_t MASK>
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t one) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(x), "n"(MASK), "r"(one));
+  return d;
+}
+
 // Sixteen codes of a stream -> 16 values of T (channels 16 c ..) as two 16-byte chunks.
 template <int BITS, typename T>
 __device__ __forceinline__ void values16(const uint32_t (&s)[(BITS + 1) / 2], const float4 (&ab)[8], float alpha,
-                                         uint4 (&out)[2]) {
+                                         uint32_t one, uint4 (&out)[2]) {
   using W = Window<BITS>;
   uint32_t x[W::kCount], r[8];
   windows<BITS>(s, x);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    float2 v;
-    v.x = __uint_as_float((x[2 * i / W::kPer] & (((1u << BITS) - 1u) << W::bit(2 * i))) | 0x3F800000u);
-    v.y = __uint_as_float((x[(2 * i + 1) / W::kPer] & (((1u << BITS) - 1u) << W::bit(2 * i + 1))) | 0x3F800000u);
+  const float2 al = make_float2(alpha, alpha);
+  constexpr uint32_t kMask = (1u << BITS) - 1u;
+  auto pair = [&](auto I) {
+    constexpr int i = decltype(I)::value;
+    const float2 v = make_float2(__uint_as_float(and_or<kMask << W::bit(2 * i)>(x[2 * i / W::kPer], one)),
+                                 __uint_as_float(and_or<kMask << W::bit(2 * i + 1)>(x[(2 * i + 1) / W::kPer], one)));
     const float2 d = tc::fma2(make_float2(ab[i].x, ab[i].y), v, make_float2(ab[i].z, ab[i].w));
-    const float2 y = tc::mul2(d, make_float2(alpha, alpha));
+    const float2 y = tc::mul2(d, al);
     r[i] = rr::round2<T>(y.x, y.y);
-  }
+  };
+  pair(Int<0>{}), pair(Int<1>{}), pair(Int<2>{}), pair(Int<3>{});
+  pair(Int<4>{}), pair(Int<5>{}), pair(Int<6>{}), pair(Int<7>{});
   out[0] = make_uint4(r[0], r[1], r[2], r[3]);
   out[1] = make_uint4(r[4], r[5], r[6], r[7]);
 }
@@ -107,7 +127,6 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
   extern __shared__ uint8_t smem_raw[];
   using R = rr::Rec<BITS>;
   using Sm = Smem<BITS>;
-  constexpr int kR = kRaw<BITS>;
   // the swizzle's pattern repeats every 1024 bytes of the shared address
   Sm &S = *reinterpret_cast<Sm *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t{1023});
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -125,12 +144,12 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
   if (warp == 16) {
     tc::tmem_alloc(&S.tmem, 512);
   } else if (tid == 0) {
-    for (int i = 0; i < kR; ++i) {
+    for (int i = 0; i < kRawWide<BITS>; ++i) {
       mbar_init(&S.raw_full[i], 1);
-      mbar_init(&S.raw_empty[i], 8);
+      mbar_init(&S.raw_empty[i], 1);
     }
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(&S.full[i], 8);
+      mbar_init(&S.full[i], 1);
       mbar_init(&S.empty[i], 1);
     }
     for (int t = 0; t < 2; ++t) {
@@ -148,17 +167,24 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
   __syncthreads();
   tc::fence_after();
   const uint32_t tmem = S.tmem;
+  const uint32_t kR = (blockIdx.z % a.pairs) * int64_t{2 * kM} + kM < nrows ? kRaw<BITS> : kRawWide<BITS>;
+  auto raw = [&](uint32_t slot) {
+    return slot < kRaw<BITS> ? S.raw[slot] : S.q[1] + (slot - kRaw<BITS>) * R::kBytes;
+  };
 
   // More row tiles than the grid has: the CTA takes every pairs-th pair of the group in turn.
   // Ring positions and parities run on from one to the next.
   uint32_t blocks = 0, pair_n = 0;  // blocks and pairs taken so far
+  uint32_t taken[2] = {0, 0};       // blocks that each softmax team has taken so far
   for (int64_t row0 = (blockIdx.z % a.pairs) * int64_t{2 * kM}; row0 < nrows;
        row0 += static_cast<int64_t>(a.pairs) * 2 * kM, blocks += nloc, ++pair_n) {
     const int tiles = row0 + kM < nrows ? 2 : 1;  // row tiles of this pair
+    const bool split = tiles == 1;                // the teams share one tile
+    const int team_blocks[2] = {split ? (nloc + 1) / 2 : nloc, split ? nloc / 2 : nloc};
     if (warp < 8) {  // ---- Q, softmax, output
       const int t = warp >> 2;
+      const int64_t first = row0 + (split ? 0 : t * kM);
       if (t < tiles) {
-        const int64_t first = row0 + t * kM;
         // Q of the tile into its swizzled place: 16 threads per row
         int bad = 0;
 #pragma unroll 4
@@ -184,15 +210,22 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
         tc::fence_async();
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(&S.q_full[t]);
-
+      }
+      {
         constexpr float kSc = kScale * fm::kLog2e;
         const uint32_t lane_base = tmem + (static_cast<uint32_t>(warp & 3) << 21);
         const uint32_t o_at = lane_base + 256 + 128 * t;
         float m = -INFINITY, base = 0.f, l = 0.f;
+        const bool rows_here = first + 32 * (warp & 3) < nrows;
 #pragma unroll 1
-        for (int j = 0; j < nloc; ++j) {
-          const uint32_t n = blocks + j, s_at = lane_base + 128 * t + 64 * (n & 1);
-          tc::wait(&S.s_full[t][n & 1], n >> 1 & 1, &S.failed, a.status);
+        for (int j = 0; j < team_blocks[t]; ++j) {
+          const uint32_t n = taken[t] + j, s_at = lane_base + 128 * t + 64 * (n & 1);
+          if (!rows_here) {  // none of this warp's rows exist: their P may be anything
+            tc::spin(&S.s_full[t][n & 1], n >> 1 & 1, &S.failed, a.status);
+            if (lane == 0) tc::mbar_arrive(&S.p_full[t][n & 1]);
+            continue;
+          }
+          tc::spin(&S.s_full[t][n & 1], n >> 1 & 1, &S.failed, a.status);
           tc::fence_after();
           float s[64];
           auto fetch = [&] {
@@ -218,10 +251,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
           for (int again = j == 0;; again = 1) {
             fetch();
             if (again) {
-              const float m_new = fmaxf(m, top());
+              const float m_new = fmaxf(m, top() + kHeadroom);
               const float c = m_new == -INFINITY ? 1.f : fm::ex2(m - m_new);
               if (j > 0) {
-                tc::wait(&S.o_done[t], (n - 1) & 1, &S.failed, a.status);  // P.V of the block before
+                tc::spin(&S.o_done[t], (n - 1) & 1, &S.failed, a.status);  // P.V of the block before
                 tc::fence_after();
 #pragma unroll 1
                 for (int i = 0; i < 8; ++i) {
@@ -258,7 +291,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
           __syncwarp();
           if (lane == 0) tc::mbar_arrive(&S.p_full[t][n & 1]);
         }
-        tc::wait(&S.o_done[t], (blocks + nloc - 1) & 1, &S.failed, a.status);
+        if (team_blocks[t]) tc::spin(&S.o_done[t], (taken[t] + team_blocks[t] - 1) & 1, &S.failed, a.status);
         tc::fence_after();
         const int64_t r = first + (tid & 127);
         int64_t qr = -1;
@@ -268,95 +301,136 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
         }
         const bool mine = qr >= 0 && qr < a.rows;
         const int64_t at = (blockIdx.x * a.rows + qr) * a.hq + head * G + r % G;
-        const float inv = m == -INFINITY ? 0.f : __fdiv_rn(1.f, l);
+        float inv = m == -INFINITY ? 0.f : __fdiv_rn(1.f, l), e2 = m == -INFINITY ? -INFINITY : m + log2f(l);
+        // Team 1's half of a shared tile goes through shared memory (Q's place: every S is done,
+        // each team having seen its last P.V), column by column of all rows.
+        float *other = reinterpret_cast<float *>(S.q) + (tid & 127);
+        float w = 0.f;
+        if (split) tc::bar_named(3, 256);
+        if (split && t == 0) {
+          tc::bar_named(4, 256);
+          const float e1 = S.e_other[tid & 127], top = fmaxf(e2, e1), b0 = top == -INFINITY ? 0.f : top;
+          const float x0 = e2 == -INFINITY ? 0.f : fm::ex2(e2 - b0), x1 = e1 == -INFINITY ? 0.f : fm::ex2(e1 - b0);
+          const float is = top == -INFINITY ? 0.f : __fdiv_rn(1.f, x0 + x1);
+          inv *= x0 * is;
+          w = x1 * is;
+          e2 = top == -INFINITY ? -INFINITY : top + log2f(x0 + x1);
+        }
+        if (!split || t == 0 || team_blocks[1]) {
 #pragma unroll 1
-        for (int i = 0; i < 4; ++i) {
-          float o[32];
-          tc::ld32(o, o_at + 32 * i);
-          tc::wait_ld();
-          tc::pin32(o);
+          for (int i = 0; i < 4; ++i) {
+            float o[32];
+            tc::ld32(o, o_at + 32 * i);
+            tc::wait_ld();
+            tc::pin32(o);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] *= inv;
-          if (mine)
+            for (int e = 0; e < 32; ++e) o[e] *= inv;
+            if (split && t == 1) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              tc::store32(a.o_ws + at * kDim + 32 * i + 8 * e, reinterpret_cast<uint32_t *>(o) + 8 * e);
+              for (int e = 0; e < 32; ++e) other[(32 * i + e) * kM] = o[e];
+              continue;
+            }
+            if (w != 0.f) {  // (NaN passes)
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = fmaf(w, other[(32 * i + e) * kM], o[e]);
+            }
+            if (mine)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                tc::store32(a.o_ws + at * kDim + 32 * i + 8 * e, reinterpret_cast<uint32_t *>(o) + 8 * e);
+          }
         }
         tc::fence_before();
-        if (mine) a.e_ws[at] = m == -INFINITY ? -INFINITY : m + log2f(l);
+        if (split && t == 1) {
+          S.e_other[tid & 127] = e2;
+          tc::bar_named(4, 256);
+        } else if (mine) {
+          a.e_ws[at] = e2;
+        }
       }
     } else if (warp < 16) {  // ---- restore
-      const int w8 = warp - 8, g16 = (w8 & 1) * 4 + (lane >> 3), r8 = (w8 >> 1) * 8 + (lane & 7);
-      const int ch = tid & 127, is_v = (tid >> 7) & 1;  // this thread's channel of the a, b tables (tid 256..511)
+      // Two teams of four warps take alternate blocks, so that one works while the other waits
+      // for its record, its tables or a free stage.
+      const int team = (warp - 8) >> 2, w4 = warp & 3;
+      const int g16 = (w4 & 1) * 4 + (lane >> 3), r8 = (w4 >> 1) * 8 + (lane & 7);
+      const int ch = tid & 127;                          // this thread's channel of the a, b tables
       const uint32_t sel = g16 & 1 ? 0x7632u : 0x5410u;  // K: this 16-channel stream's halves of the words
+      // this thread's codes in a record and rows in a stage: K tokens r8 + 16 e, V tokens 2 r8 + 32 e
+      // and 2 r8 + 32 e + 1 (whose swizzle exchanges the two chunks)
+      const int k_src = (r8 * 4 * BITS + (g16 >> 1) * BITS) * 4, v_src = R::kHalf + (r8 * 8 + g16) * BITS * 4;
+      const int k_dst = chunk_at(r8, 2 * g16), v_dst = kRowsBytes + chunk_at(2 * r8, 2 * g16);
+      const float mul = __int_as_float((127 + 23 - Window<BITS>::bit(ch & 15)) << 23);
+      uint32_t one;
+      asm volatile("mov.u32 %0, 0x3F800000;" : "=r"(one));  // kept in a register
+      const int mine = team ^ (blocks & 1);                 // the first block of this chunk that is the team's
+      uint32_t slot = (blocks + mine) % kR, raw_par = (blocks + mine) / kR & 1;
+      uint32_t stage = (blocks + mine) % kStages, par = (blocks + mine) / kStages & 1;
       int bad = 0;
 #pragma unroll 1
-      for (int j = 0; j < nloc; ++j) {
-        const uint32_t n = blocks + j, slot = n % kR, stage = n % kStages;
-        const uint8_t *rec = S.raw[slot];
-        tc::wait(&S.raw_full[slot], n / kR & 1, &S.failed, a.status);
-        {
-          const uint8_t *half = rec + is_v * R::kHalf;
-          const float mn = half_bits_to_f(reinterpret_cast<const uint16_t *>(half + R::kMin)[ch]);
-          const float sc = half_bits_to_f(reinterpret_cast<const uint16_t *>(half + R::kScaleAt)[ch]);
-          bad |= !isfinite(mn) || !isfinite(sc);
-          using W = Window<BITS>;
-          const int i = ch & 15, bit = W::kAt + BITS * (i % W::kPer);
-          const float x = sc * __int_as_float((127 + 23 - bit) << 23);
-          // pairs of channels as (a, a, b, b)
-          float *dst = reinterpret_cast<float *>(&S.ab[n & 1][is_v][ch & ~1]) + (ch & 1);
-          dst[0] = x;
-          dst[2] = mn - x;
+      for (int j = mine; j < nloc; j += 2) {
+        const uint8_t *rec = raw(slot);
+        tc::spin(&S.raw_full[slot], raw_par, &S.failed, a.status);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {  // K, V; channel pairs as (a, a, b, b)
+          const uint16_t *half = reinterpret_cast<const uint16_t *>(rec + x * R::kHalf + R::kMin) + ch;
+          const float mn = half_bits_to_f(half[0]), sc = half_bits_to_f(half[128]), p = sc * mul, y = mn - p;
+          bad |= !isfinite(y);
+          float *dst = reinterpret_cast<float *>(&S.ab[team][x][ch & ~1]) + (ch & 1);
+          dst[0] = p;
+          dst[2] = y;
         }
-        tc::bar_named(1, 256);
-        tc::wait(&S.empty[stage], (n / kStages & 1) ^ 1, &S.failed, a.status);
+        tc::bar_named(1 + team, 128);
+        tc::spin(&S.empty[stage], par ^ 1, &S.failed, a.status);
+        uint8_t *rows = S.kv[stage][0];
+        const float4 *tab = reinterpret_cast<const float4 *>(S.ab[team][0]) + 8 * g16;
         float4 ab[8];
         uint4 out[2];
         uint32_t st[(BITS + 1) / 2], wd[BITS];
-        const float4 *tab = reinterpret_cast<const float4 *>(S.ab[n & 1][0]) + 8 * g16;
 #pragma unroll
         for (int i = 0; i < 8; ++i) ab[i] = tab[i];
-#pragma unroll 1
-        for (int e = 0; e < 2; ++e) {  // K: token r8 + 32 e
-          const int t = r8 + 32 * e;
-          const uint32_t *src = reinterpret_cast<const uint32_t *>(rec) + t * 4 * BITS + (g16 >> 1) * BITS;
-          const float alpha = reinterpret_cast<const float *>(rec + R::kAlpha)[t];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t *src = reinterpret_cast<const uint32_t *>(rec + k_src + e * 16 * 16 * BITS);
+          const float alpha = reinterpret_cast<const float *>(rec + R::kAlpha)[r8 + 16 * e];
           bad |= !isfinite(alpha);
 #pragma unroll
           for (int i = 0; i < BITS; ++i) wd[i] = src[i];
 #pragma unroll
           for (int i = 0; i < (BITS + 1) / 2; ++i)
             st[i] = __byte_perm(wd[2 * i], 2 * i + 1 < BITS ? wd[2 * i + 1] : 0u, sel);
-          values16<BITS, T>(st, ab, alpha, out);
-          *reinterpret_cast<uint4 *>(S.kv[stage][0] + chunk_at(t, 2 * g16)) = out[0];
-          *reinterpret_cast<uint4 *>(S.kv[stage][0] + chunk_at(t, 2 * g16 + 1)) = out[1];
+          values16<BITS, T>(st, ab, alpha, one, out);
+          *reinterpret_cast<uint4 *>(rows + k_dst + e * 16 * 128) = out[0];
+          *reinterpret_cast<uint4 *>(rows + (k_dst ^ 16) + e * 16 * 128) = out[1];
         }
-        tab = reinterpret_cast<const float4 *>(S.ab[n & 1][1]) + 8 * g16;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ab[i] = tab[i];
-        {  // V: tokens 2 r8 and 2 r8 + 1
-          const uint32_t *src = reinterpret_cast<const uint32_t *>(rec + R::kHalf) + r8 * 8 * BITS + g16 * BITS;
-          const float2 alpha = reinterpret_cast<const float2 *>(rec + R::kHalf + R::kAlpha)[r8];
+        for (int i = 0; i < 8; ++i) ab[i] = tab[i + kDim / 2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t *src = reinterpret_cast<const uint32_t *>(rec + v_src + e * 16 * 8 * BITS * 4);
+          const float2 alpha = reinterpret_cast<const float2 *>(rec + R::kHalf + R::kAlpha)[r8 + 16 * e];
           bad |= !isfinite(alpha.x) || !isfinite(alpha.y);
 #pragma unroll
           for (int i = 0; i < BITS; ++i) wd[i] = src[i];
-#pragma unroll 1
-          for (int e = 0; e < 2; ++e) {
-            const int t = 2 * r8 + e;
+          uint8_t *dst = rows + e * 32 * 128;
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
 #pragma unroll
             for (int i = 0; i < (BITS + 1) / 2; ++i)
-              st[i] = __byte_perm(wd[2 * i], 2 * i + 1 < BITS ? wd[2 * i + 1] : 0u, e ? 0x7632u : 0x5410u);
-            values16<BITS, T>(st, ab, e ? alpha.y : alpha.x, out);
-            *reinterpret_cast<uint4 *>(S.kv[stage][1] + chunk_at(t, 2 * g16)) = out[0];
-            *reinterpret_cast<uint4 *>(S.kv[stage][1] + chunk_at(t, 2 * g16 + 1)) = out[1];
+              st[i] = __byte_perm(wd[2 * i], 2 * i + 1 < BITS ? wd[2 * i + 1] : 0u, y ? 0x7632u : 0x5410u);
+            values16<BITS, T>(st, ab, y ? alpha.y : alpha.x, one, out);
+            *reinterpret_cast<uint4 *>(dst + (v_dst ^ (16 * y)) + y * 128) = out[0];
+            *reinterpret_cast<uint4 *>(dst + (v_dst ^ (16 * (1 - y))) + y * 128) = out[1];
           }
         }
         tc::fence_async();
-        __syncwarp();
-        if (lane == 0) {
+        tc::bar_named(1 + team, 128);  // the record and the tables have been read, the rows written
+        if ((tid & 127) == 0) {
           tc::mbar_arrive(&S.full[stage]);
           tc::mbar_arrive(&S.raw_empty[slot]);
         }
+        slot += 2, stage += 2;
+        if (slot >= kR) slot -= kR, raw_par ^= 1;  // kR >= 2
+        if (stage >= kStages) stage -= kStages, par ^= 1;
       }
       if (bad) set_status(a.status, NSNKV_ST_INPUT_NONFINITE);
     } else if (warp == 16) {  // ---- MMA: every lane runs the loops, one issues
@@ -365,42 +439,62 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
       const uint64_t qd = tc::smem_desc(tc::saddr(S.q[0]), 16, 1024),
                      kd = tc::smem_desc(tc::saddr(S.kv[0][0]), 16, 1024),
                      vd = tc::smem_desc(tc::saddr(S.kv[0][1]), kRowsBytes / 2, 1024);
-      auto scores = [&](uint32_t n) {  // S of block n for the pair's row tiles
-        const uint32_t stage = n % kStages;
-        tc::wait(&S.full[stage], n / kStages & 1, &S.failed, a.status);
-        tc::fence_after();
+      uint32_t cs[2] = {taken[0], taken[1]}, cp[2] = {taken[0], taken[1]};  // S and P.V issued per team
 #pragma unroll 1
-        for (int t = 0; t < tiles; ++t)
-          if (lead) {
-            const uint64_t qa = qd + t * (kM * kDim * 2 >> 4), ka = kd + stage * (2 * kRowsBytes >> 4);
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              tc::mma_ss(tmem + 128 * t + 64 * (n & 1), qa + (((i >> 2) * (kM * 128) + (i & 3) * 32) >> 4),
-                         ka + (((i >> 2) * (kRowsBytes / 2) + (i & 3) * 32) >> 4), kIdS, i > 0);
-            tc::commit(&S.s_full[t][n & 1]);
-          }
-      };
+      for (int t = 0; t < tiles; ++t) tc::spin(&S.q_full[t], pair_n & 1, &S.failed, a.status);
+      // S of block sj as soon as the block is restored and a team's buffer is free (P.V of its
+      // block there is issued), P.V of block pj as soon as its P is there: whichever comes first.
+      const int ahead = split ? 3 : 1;
+      int sj = 0, pj = 0, pt = 0;  // pt: the team whose P.V of block pj is next
 #pragma unroll 1
-      for (int t = 0; t < tiles; ++t) tc::wait(&S.q_full[t], pair_n & 1, &S.failed, a.status);
-      scores(blocks);
-#pragma unroll 1
-      for (int j = 0; j < nloc; ++j) {
-        const uint32_t n = blocks + j, stage = n % kStages;
-        if (j + 1 < nloc) scores(n + 1);
-#pragma unroll 1
-        for (int t = 0; t < tiles; ++t) {
-          tc::wait(&S.p_full[t][n & 1], n >> 1 & 1, &S.failed, a.status);
+      for (int idle = 0; pj < nloc;) {
+        const uint32_t s_stage = (blocks + sj) % kStages;
+        if (sj < nloc && sj <= pj + ahead && tc::test(&S.full[s_stage], (blocks + sj) / kStages & 1)) {
           tc::fence_after();
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            if (!split || (sj & 1) == t) {
+              if (lead) {
+                const uint64_t qa = qd + (split ? 0 : t * (kM * kDim * 2 >> 4)),
+                               ka = kd + s_stage * (2 * kRowsBytes >> 4);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                  tc::mma_ss(tmem + 128 * t + 64 * (cs[t] & 1), qa + (((i >> 2) * (kM * 128) + (i & 3) * 32) >> 4),
+                             ka + (((i >> 2) * (kRowsBytes / 2) + (i & 3) * 32) >> 4), kIdS, i > 0);
+                tc::commit(&S.s_full[t][cs[t] & 1]);
+              }
+              ++cs[t];
+            }
+          ++sj;
+          idle = 0;
+          continue;
+        }
+        const int t = split ? pj & 1 : pt;
+        const uint32_t c = t ? cp[1] : cp[0];
+        if (sj > pj && tc::test(&S.p_full[t][c & 1], c >> 1 & 1)) {
+          tc::fence_after();
+          const uint32_t stage = (blocks + pj) % kStages;
+          const bool last = split || t == 1;  // of the block's P.V
           if (lead) {
             const uint64_t va = vd + stage * (2 * kRowsBytes >> 4);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              tc::mma_ts(tmem + 256 + 128 * t, tmem + 128 * t + 64 * (n & 1) + 8 * i, va + i * (2048 >> 4), kIdO,
-                         j > 0 || i > 0);
+              tc::mma_ts(tmem + 256 + 128 * t, tmem + 128 * t + 64 * (c & 1) + 8 * i, va + i * (2048 >> 4), kIdO,
+                         pj > (split ? 1 : 0) || i > 0);
             tc::commit(&S.o_done[t]);
+            if (last) tc::commit(&S.empty[stage]);
           }
+          if (t) ++cp[1]; else ++cp[0];
+          pt = last ? 0 : 1;
+          pj += last;
+          idle = 0;
+          continue;
         }
-        if (lead) tc::commit(&S.empty[stage]);
+        if (++idle > 1 << 16) {  // neither came: give up through the bounded wait
+          tc::wait_long(&S.p_full[t][c & 1], c >> 1 & 1, &S.failed, a.status);
+          if (*static_cast<volatile int32_t *>(&S.failed)) break;
+          idle = 0;
+        }
       }
       __syncwarp();
     } else if (warp == 17) {  // ---- records
@@ -416,16 +510,17 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
           if (lead) set_status(a.status, NSNKV_ST_PAGE);
           page = 0;
         }
-        tc::wait(&S.raw_empty[slot], (n / kR & 1) ^ 1, &S.failed, a.status);
+        tc::spin(&S.raw_empty[slot], (n / kR & 1) ^ 1, &S.failed, a.status);
         if (lead) {
           mbar_expect_tx(&S.raw_full[slot], R::kBytes);
-          bulk_g2s(S.raw[slot], a.records + head * a.rec_head + page * a.rec_page, R::kBytes, &S.raw_full[slot]);
+          bulk_g2s(raw(slot), a.records + head * a.rec_head + page * a.rec_page, R::kBytes, &S.raw_full[slot]);
         }
       }
       __syncwarp();
       if (*static_cast<volatile int32_t *>(&S.failed))  // a wait gave up: let the copies in flight land
         for (int i = 0; i < 1000; ++i) __nanosleep(1000);
     }
+    taken[0] += team_blocks[0], taken[1] += team_blocks[1];
     // The next pair reuses O, the Q tiles and, where a row tile had no rows, untouched barriers.
     if (row0 + static_cast<int64_t>(a.pairs) * 2 * kM < nrows) {
       tc::fence_before();

@@ -29,6 +29,24 @@ static __device__ __noinline__ void wait_long(uint64_t *bar, uint32_t phase, vol
   *failed = 1;
   set_status(status, NSNKV_ST_TIMEOUT);
 }
+// Whether the phase is complete, without suspending the thread (as try_wait may).
+__device__ __forceinline__ bool test(uint64_t *bar, uint32_t phase) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(saddr(bar)), "r"(phase)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ void spin(uint64_t *bar, uint32_t phase, int32_t *failed, int32_t *status) {
+#pragma unroll 1
+  for (int i = 0; i < 16384; ++i)
+    if (test(bar, phase)) return;
+  wait_long(bar, phase, failed, status);
+}
 __device__ __forceinline__ void wait(uint64_t *bar, uint32_t phase, int32_t *failed, int32_t *status) {
 #pragma unroll 1
   for (int i = 0; i < 4096; ++i)

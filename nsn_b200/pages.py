@@ -15,18 +15,18 @@ import torch
 
 from . import _lib as L
 from . import primitives as w
-from .kernel import workspace
+
+_ARRAYS = {n: L.PageArray * n for n in range(1, 9)}
 
 
-def _ints(name, *tensors):
-    dev = tensors[0].device
-    w.require(all(t.is_cuda and t.device == dev and t.dtype == torch.int32 and (t.numel() == 0 or t.stride(-1) == 1)
-                  for t in tensors), f"{name}: int32 CUDA tensors on one device")
-    return dev
+def _ints(name, dev, *tensors):
+    for t in tensors:
+        if not (t.dtype == torch.int32 and t.device == dev and t.is_cuda and (t.numel() <= 1 or t.stride(-1) == 1)):
+            raise w.ContractError(f"{name}: int32 CUDA tensors on one device")
 
 
 def _p(t):
-    return t.data_ptr() if t is not None else None
+    return None if t is None else t.data_ptr()
 
 
 def fork_sequences(block_table, n_blocks, tail_len, page_refs, k_tail, v_tail, src, dst, status=None):
@@ -37,36 +37,35 @@ def fork_sequences(block_table, n_blocks, tail_len, page_refs, k_tail, v_tail, s
     [count] are int32, the tails [batch, h, 64, 128] fp16 or bf16; all change in place.  The dst
     are distinct sequences and none of them is a src.
     """
-    dev = _ints("fork_sequences", block_table, n_blocks, tail_len, page_refs, src, dst)
-    batch = block_table.shape[0]
-    w.require(block_table.ndim == 2 and n_blocks.shape == (batch,) and tail_len.shape == (batch,)
-              and src.ndim == 1 and src.shape == dst.shape, "fork_sequences tables")
-    w.require(k_tail.ndim == 4 and k_tail.shape == v_tail.shape and k_tail.shape[0] == batch
-              and k_tail.shape[2:] == (w.BLOCK, w.DIM) and k_tail.dtype == v_tail.dtype
-              and k_tail.dtype in (torch.float16, torch.bfloat16) and k_tail.is_contiguous() and v_tail.is_contiguous()
-              and k_tail.device == dev and v_tail.device == dev, "fork_sequences tails [batch, h, 64, 128]")
-    h = k_tail.shape[1]
-    with torch.cuda.device(dev):
-        rc = L.load().nsnkv_fork_sequences(
-            batch, h, page_refs.numel(), block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
-            n_blocks.data_ptr(), tail_len.data_ptr(), page_refs.data_ptr(), k_tail.data_ptr(), v_tail.data_ptr(),
-            h * w.BLOCK, w.BLOCK, src.numel(), src.data_ptr(), dst.data_ptr(), _p(status),
-            torch.cuda.current_stream(dev).cuda_stream)
+    dev, (batch, max_blocks) = block_table.device, block_table.shape
+    _ints("fork_sequences", dev, block_table, n_blocks, tail_len, page_refs, src, dst)
+    kt = k_tail.shape
+    if not (n_blocks.shape == tail_len.shape == (batch,) and src.ndim == 1 and src.shape == dst.shape
+            and page_refs.ndim == 1):
+        raise w.ContractError("fork_sequences tables: block_table [batch, max_blocks], counters [batch], src, dst [count]")
+    if not (len(kt) == 4 and kt[0] == batch and kt[2] == w.BLOCK and kt[3] == w.DIM and v_tail.shape == kt
+            and k_tail.dtype == v_tail.dtype and k_tail.dtype in (torch.float16, torch.bfloat16)
+            and k_tail.is_contiguous() and v_tail.is_contiguous() and k_tail.device == dev and v_tail.device == dev):
+        raise w.ContractError("fork_sequences tails: contiguous [batch, h, 64, 128] fp16 or bf16")
+    index, h = dev.index, kt[1]
+    rc = L.call_on(index, L.load().nsnkv_fork_sequences, batch, h, page_refs.shape[0], block_table.data_ptr(),
+                   block_table.stride(0), max_blocks, n_blocks.data_ptr(), tail_len.data_ptr(), page_refs.data_ptr(),
+                   k_tail.data_ptr(), v_tail.data_ptr(), h * w.BLOCK, w.BLOCK, src.shape[0], src.data_ptr(),
+                   dst.data_ptr(), _p(status), L.raw_stream(index))
     if rc:
         L.check(rc, "nsnkv_fork_sequences")
 
 
 def free_sequences(block_table, n_blocks, tail_len, page_refs, seqs, status=None):
     """Sequences ``seqs`` (int32 [count]) drop their pages and are empty; in place."""
-    dev = _ints("free_sequences", block_table, n_blocks, tail_len, page_refs, seqs)
-    batch = block_table.shape[0]
-    w.require(block_table.ndim == 2 and n_blocks.shape == (batch,) and tail_len.shape == (batch,) and seqs.ndim == 1,
-              "free_sequences tables")
-    with torch.cuda.device(dev):
-        rc = L.load().nsnkv_free_sequences(
-            batch, page_refs.numel(), block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
-            n_blocks.data_ptr(), tail_len.data_ptr(), page_refs.data_ptr(), seqs.numel(), seqs.data_ptr(), _p(status),
-            torch.cuda.current_stream(dev).cuda_stream)
+    dev, (batch, max_blocks) = block_table.device, block_table.shape
+    _ints("free_sequences", dev, block_table, n_blocks, tail_len, page_refs, seqs)
+    if not (n_blocks.shape == tail_len.shape == (batch,) and seqs.ndim == 1 and page_refs.ndim == 1):
+        raise w.ContractError("free_sequences tables: block_table [batch, max_blocks], counters [batch], seqs [count]")
+    index = dev.index
+    rc = L.call_on(index, L.load().nsnkv_free_sequences, batch, page_refs.shape[0], block_table.data_ptr(),
+                   block_table.stride(0), max_blocks, n_blocks.data_ptr(), tail_len.data_ptr(), page_refs.data_ptr(),
+                   seqs.shape[0], seqs.data_ptr(), _p(status), L.raw_stream(index))
     if rc:
         L.check(rc, "nsnkv_free_sequences")
 
@@ -75,40 +74,51 @@ def reserve_pages(block_table, n_blocks, page_refs, ahead=1, status=None):
     """Pages for every sequence's next ``ahead`` blocks where its table entries name none, in
     place: in (sequence, entry) order they take the free pages in ascending order.  ``status`` gets
     NSNKV_ST_CAPACITY when too few pages are free; the entries left over stay unassigned."""
-    dev = _ints("reserve_pages", block_table, n_blocks, page_refs)
-    batch = block_table.shape[0]
-    w.require(block_table.ndim == 2 and n_blocks.shape == (batch,), "reserve_pages tables")
-    with torch.cuda.device(dev):
-        rc = L.load().nsnkv_reserve_pages(
-            batch, page_refs.numel(), block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
-            n_blocks.data_ptr(), page_refs.data_ptr(), int(ahead), _p(status),
-            torch.cuda.current_stream(dev).cuda_stream)
+    dev, (batch, max_blocks) = block_table.device, block_table.shape
+    _ints("reserve_pages", dev, block_table, n_blocks, page_refs)
+    if not (n_blocks.shape == (batch,) and page_refs.ndim == 1):
+        raise w.ContractError("reserve_pages tables: block_table [batch, max_blocks], n_blocks [batch]")
+    index = dev.index
+    rc = L.call_on(index, L.load().nsnkv_reserve_pages, batch, page_refs.shape[0], block_table.data_ptr(),
+                   block_table.stride(0), max_blocks, n_blocks.data_ptr(), page_refs.data_ptr(), int(ahead), _p(status),
+                   L.raw_stream(index))
     if rc:
         L.check(rc, "nsnkv_reserve_pages")
 
 
 def _page_arrays(arrays, dev):
     """[h, pages, ...] tensors as nsnkv_page_array descriptors: (h, pages, ctypes array)."""
-    w.require(0 < len(arrays) <= 8 and all(t.ndim >= 3 and t.shape[:2] == arrays[0].shape[:2] and t.device == dev
-                                           for t in arrays), "page arrays: one to eight [h, pages, ...] tensors")
-    got = (L.PageArray * len(arrays))()
-    for d, t in zip(got, arrays):
-        size = t.element_size()
-        w.require(t[0, 0].is_contiguous(), "page arrays: contiguous pages")
-        d.base, d.bytes = t.data_ptr(), t[0, 0].numel() * size
-        d.stride_head, d.stride_page = t.stride(0) * size, t.stride(1) * size
-    return arrays[0].shape[0], arrays[0].shape[1], got
+    got = _ARRAYS[len(arrays)]() if 0 < len(arrays) <= 8 else None
+    lead = arrays[0].shape[:2] if got is not None else None
+    for i, t in enumerate(arrays):
+        shape, stride, size = t.shape, t.stride(), t.element_size()
+        n = size
+        for d in range(len(shape) - 1, 1, -1):  # contiguous pages
+            if stride[d] * size != n and shape[d] != 1:
+                n = -1
+                break
+            n *= shape[d]
+        if got is None or len(shape) < 3 or shape[:2] != lead or t.device != dev or n <= 0:
+            got = None
+            break
+        a = got[i]
+        a.base, a.bytes, a.stride_head, a.stride_page = t.data_ptr(), n, stride[0] * size, stride[1] * size
+    if got is None:
+        raise w.ContractError("page arrays: one to eight [h, pages, ...] tensors of one device with contiguous pages")
+    return lead[0], lead[1], got
 
 
 def copy_pages(arrays, src, dst, status=None):
     """Page dst[i] of every array ([h, pages, ...] tensors of a pool) becomes a copy of page
     src[i], for all heads (src, dst int32 [count]; no dst is the src of another pair)."""
-    dev = _ints("copy_pages", src, dst)
-    w.require(src.ndim == 1 and src.shape == dst.shape, "copy_pages src, dst")
+    dev = src.device
+    _ints("copy_pages", dev, src, dst)
+    if src.ndim != 1 or src.shape != dst.shape:
+        raise w.ContractError("copy_pages src, dst: int32 [count]")
     h, pages, arr = _page_arrays(arrays, dev)
-    with torch.cuda.device(dev):
-        rc = L.load().nsnkv_copy_pages(h, pages, len(arrays), arr, src.numel(), src.data_ptr(), dst.data_ptr(),
-                                       _p(status), torch.cuda.current_stream(dev).cuda_stream)
+    index = dev.index
+    rc = L.call_on(index, L.load().nsnkv_copy_pages, h, pages, len(arrays), arr, src.shape[0], src.data_ptr(),
+                   dst.data_ptr(), _p(status), L.raw_stream(index))
     if rc:
         L.check(rc, "nsnkv_copy_pages")
 
@@ -122,25 +132,25 @@ def compact_pages(arrays, block_table, page_refs, table_out=None, refs_out=None,
     (table [batch, max_blocks], refs [pages], live int32 [1]): the block table and counts of the
     moved pages and L, in new tensors or in ``table_out`` / ``refs_out`` (which may be the inputs).
     """
-    dev = _ints("compact_pages", block_table, page_refs)
-    h, pages, arr = _page_arrays(arrays, dev)
-    w.require(block_table.ndim == 2 and page_refs.shape == (pages,), "compact_pages tables")
+    dev, (batch, max_blocks) = block_table.device, block_table.shape
     if table_out is None:
-        table_out = torch.empty(block_table.shape, dtype=torch.int32, device=dev)
+        table_out = torch.empty((batch, max_blocks), dtype=torch.int32, device=dev)
     if refs_out is None:
         refs_out = torch.empty_like(page_refs)
     live = torch.empty(1, dtype=torch.int32, device=dev)
-    _ints("compact_pages outputs", table_out, refs_out, live)
-    w.require(table_out.shape == block_table.shape and refs_out.shape == page_refs.shape, "compact_pages outputs")
-    lib = L.load()
+    _ints("compact_pages", dev, block_table, page_refs, table_out, refs_out)
+    h, pages, arr = _page_arrays(arrays, dev)
+    if not (page_refs.shape == refs_out.shape == (pages,) and table_out.shape == block_table.shape):
+        raise w.ContractError("compact_pages tables: block_table and table_out [batch, max_blocks], page_refs and "
+                              "refs_out [pages]")
+    lib, index = L.load(), dev.index
+    stream = L.raw_stream(index)
     if ws is None:
-        ws = workspace(lib.nsnkv_compact_pages_workspace_bytes(pages), dev)
-    with torch.cuda.device(dev):
-        rc = lib.nsnkv_compact_pages(
-            h, pages, len(arrays), arr, block_table.shape[0], block_table.shape[1], block_table.data_ptr(),
-            block_table.stride(0), table_out.data_ptr(), table_out.stride(0), page_refs.data_ptr(),
-            refs_out.data_ptr(), live.data_ptr(), ws.data_ptr(), ws.numel(), _p(status),
-            torch.cuda.current_stream(dev).cuda_stream)
+        ws = L.scratch(lib.nsnkv_compact_pages_workspace_bytes(pages), dev, stream)
+    rc = L.call_on(index, lib.nsnkv_compact_pages, h, pages, len(arrays), arr, batch, max_blocks,
+                   block_table.data_ptr(), block_table.stride(0), table_out.data_ptr(), table_out.stride(0),
+                   page_refs.data_ptr(), refs_out.data_ptr(), live.data_ptr(), ws.data_ptr(), ws.numel(), _p(status),
+                   stream)
     if rc:
         L.check(rc, "nsnkv_compact_pages")
     return table_out, refs_out, live

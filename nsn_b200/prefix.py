@@ -12,7 +12,14 @@ import torch
 
 from . import _lib as L
 from . import primitives as w
-from .kernel import workspace
+
+_TYPES = {torch.float16: L.F16, torch.bfloat16: L.BF16}
+_RECORD = {bits: 2 * (w.code_bytes(bits) + 768) for bits in (3, 5)}
+
+
+def _ints(t, n, dev):
+    return t is None or (t.dtype == torch.int32 and t.ndim == 1 and t.shape[0] == n and t.device == dev
+                         and t.is_contiguous())
 
 
 def prefix_attention(q, records, page_table, n_pages=None, *, bits=3, row_offsets=None, row_index=None, max_rows=None,
@@ -33,45 +40,50 @@ def prefix_attention(q, records, page_table, n_pages=None, *, bits=3, row_offset
     NSNKV_ST_* bits of nsnkv_prefix_attn.  ``ws``: scratch of at least
     nsnkv_prefix_attn_workspace_bytes (default: one buffer per stream).  No host sync.
     """
-    dt, dev = q.dtype, q.device
-    rows, hq = q.shape[0], q.shape[1] if q.ndim == 3 else 0
-    w.require(q.ndim == 3 and q.shape[2] == w.DIM and dt in L.DTYPE_CODE and dt is not torch.float32
-              and q.is_contiguous() and q.is_cuda, "prefix attention q: contiguous [rows, hq, 128] fp16 or bf16 on CUDA")
-    w.require(records.dtype == torch.uint8 and records.ndim == 3 and records.stride(2) == 1 and bits in (3, 5)
-              and records.shape[2] == 2 * (w.code_bytes(bits) + 768) and hq % max(1, records.shape[0]) == 0
-              and hq > 0 and not (records.stride(0) | records.stride(1)) & 15,
-              "prefix attention records: [h, pages, record] uint8 block records of INT3 or INT5, hq a multiple of h")
+    dt, dev, qs, rs = q.dtype, q.device, q.shape, records.shape
+    rows, hq = (qs[0], qs[1]) if len(qs) == 3 else (0, 0)
+    if not (hq > 0 and qs[2] == w.DIM and dt in _TYPES and q.is_contiguous() and q.is_cuda):
+        raise w.ContractError("prefix attention q: contiguous [rows, hq, 128] fp16 or bf16 on CUDA")
+    if not (len(rs) == 3 and rs[2] == _RECORD.get(bits) and rs[0] > 0 and hq % rs[0] == 0
+            and records.dtype == torch.uint8 and records.device == dev):
+        raise w.ContractError("prefix attention records: [h, pages, record] uint8 block records of INT3 or INT5 on q's "
+                              "device, hq a multiple of h")
+    head, page, byte = records.stride()
+    if byte != 1 or (head | page) & 15:
+        raise w.ContractError("prefix attention records: contiguous records, strides multiples of 16")
     table = page_table if page_table.ndim == 2 else page_table[None]
     groups, max_pages = table.shape
-    ints = [t for t in (table, n_pages, row_offsets, row_index) if t is not None]
-    w.require(all(t.dtype == torch.int32 and t.device == dev and (t.numel() == 0 or t.stride(-1) == 1) for t in ints)
-              and records.device == dev, "prefix attention tables: int32 on q's device")
-    w.require((n_pages is None or n_pages.shape == (groups,)) and (row_index is None or row_index.shape == (rows,))
-              and (row_offsets.shape == (groups + 1,) if row_offsets is not None else groups == 1),
-              "prefix attention groups: n_pages [groups], row_offsets [groups + 1], row_index [rows]")
-    w.require((o_part is None) == (lse_part is None) and
-              (o_part is None or (o_part.shape == q.shape and lse_part.shape == (rows, hq)
-                                  and o_part.dtype == lse_part.dtype == torch.float32 and o_part.is_contiguous()
-                                  and lse_part.is_contiguous() and o_part.device == dev and lse_part.device == dev)),
-              "prefix attention partial: fp32 o_part [rows, hq, 128] with lse_part [rows, hq]")
+    if not (table.dtype == torch.int32 and table.device == dev and (max_pages <= 1 or table.stride(1) == 1)
+            and _ints(n_pages, groups, dev) and _ints(row_index, rows, dev) and _ints(row_offsets, groups + 1, dev)
+            and (row_offsets is not None or groups == 1)):
+        raise w.ContractError("prefix attention tables: int32 on q's device: page_table [groups, max_pages], n_pages "
+                              "[groups], row_offsets [groups + 1] (needed with groups), row_index [rows]")
+    o_ptr = e_ptr = None
+    if o_part is not None or lse_part is not None:
+        if not (o_part is not None and lse_part is not None and o_part.shape == qs and lse_part.shape == qs[:2]
+                and o_part.dtype == lse_part.dtype == torch.float32 and o_part.is_contiguous()
+                and lse_part.is_contiguous() and o_part.device == dev and lse_part.device == dev):
+            raise w.ContractError("prefix attention partial: fp32 o_part [rows, hq, 128] with lse_part [rows, hq]")
+        o_ptr, e_ptr = o_part.data_ptr(), lse_part.data_ptr()
     if out is None:
-        out = torch.empty_like(q)
+        out = torch.empty(qs, dtype=dt, device=dev)
+    elif not (out.shape == qs and out.dtype == dt and out.is_contiguous() and out.device == dev):
+        raise w.ContractError("prefix attention out: contiguous, of q's shape, dtype and device")
     if lse is None:
         lse = torch.empty((rows, hq), dtype=torch.float32, device=dev)
-    w.require(out.shape == q.shape and out.dtype == dt and out.is_contiguous() and lse.shape == (rows, hq)
-              and lse.dtype == torch.float32 and lse.is_contiguous() and out.device == dev and lse.device == dev,
-              "prefix attention outputs")
-    lib, h = L.load(), records.shape[0]
-    need = lib.nsnkv_prefix_attn_workspace_bytes(rows, groups, hq, h, max_pages)
+    elif not (lse.shape == qs[:2] and lse.dtype == torch.float32 and lse.is_contiguous() and lse.device == dev):
+        raise w.ContractError("prefix attention lse: contiguous fp32 [rows, hq] on q's device")
+    lib, index = L.load(), dev.index
+    stream = L.raw_stream(index)
     if ws is None:
-        ws = workspace(need, dev)
-    p = lambda t: t.data_ptr() if t is not None else None
-    with torch.cuda.device(dev):
-        rc = lib.nsnkv_prefix_attn(
-            rows, groups, int(max_rows or 0), hq, h, bits, L.DTYPE_CODE[dt], q.data_ptr(), records.data_ptr(),
-            records.shape[1], records.stride(0), records.stride(1), table.data_ptr(), table.stride(0), p(n_pages),
-            max_pages, p(row_offsets), p(row_index), p(o_part), p(lse_part), out.data_ptr(), lse.data_ptr(),
-            ws.data_ptr(), ws.numel(), p(status), torch.cuda.current_stream(dev).cuda_stream)
+        ws = L.scratch(lib.nsnkv_prefix_attn_workspace_bytes(rows, groups, hq, rs[0], max_pages), dev, stream)
+    rc = L.call_on(
+        index, lib.nsnkv_prefix_attn, rows, groups, int(max_rows or 0), hq, rs[0], bits, _TYPES[dt], q.data_ptr(),
+        records.data_ptr(), rs[1], head, page, table.data_ptr(), table.stride(0),
+        None if n_pages is None else n_pages.data_ptr(), max_pages,
+        None if row_offsets is None else row_offsets.data_ptr(), None if row_index is None else row_index.data_ptr(),
+        o_ptr, e_ptr, out.data_ptr(), lse.data_ptr(), ws.data_ptr(), ws.numel(),
+        None if status is None else status.data_ptr(), stream)
     if rc:
         L.check(rc, "nsnkv_prefix_attn")
     return out, lse

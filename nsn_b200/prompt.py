@@ -11,6 +11,8 @@ import torch
 from . import _lib as L
 from . import primitives as w
 
+_TYPES = {torch.float16: L.F16, torch.bfloat16: L.BF16}
+
 
 def prompt_attention(q, k, v, cu_seqlens, max_seqlen, *, causal=True, out=None, lse=None, status=None):
     """Attention of q [T, hq, 128] over k, v [T, h, 128] (fp16 or bf16) within each sequence
@@ -23,32 +25,33 @@ def prompt_attention(q, k, v, cu_seqlens, max_seqlen, *, causal=True, out=None, 
     NSNKV_ST_OUTPUT_NONFINITE is OR-ed in when an output is not finite.  No host sync.
     """
     dt, dev = q.dtype, q.device
-    ok = (q.ndim == 3 and k.ndim == 3 and dt in L.DTYPE_CODE and dt is not torch.float32 and q.shape[2] == w.DIM
-          and k.shape == v.shape and k.shape[0] == q.shape[0] and k.shape[2] == w.DIM and k.dtype == dt
-          and v.dtype == dt and k.shape[1] > 0 and q.shape[1] % k.shape[1] == 0)
-    w.require(ok, "prompt attention operands: q [T, hq, 128], k and v [T, h, 128], fp16 or bf16, hq a multiple of h")
-    w.require(cu_seqlens.dtype == torch.int32 and cu_seqlens.ndim == 1 and cu_seqlens.numel() > 0
-              and cu_seqlens.is_contiguous(), "prompt attention cu_seqlens: contiguous int32 [seqs + 1]")
-    w.require(q.is_cuda and k.device == dev and v.device == dev and cu_seqlens.device == dev,
-              "prompt attention operands on one CUDA device")
+    qs, ks = q.shape, k.shape
+    T, hq, h = (qs[0], qs[1], ks[1]) if len(qs) == 3 and len(ks) == 3 else (0, 0, 0)
+    if not (h > 0 and hq % h == 0 and qs[2] == ks[2] == w.DIM and ks[0] == T and v.shape == ks and k.dtype == dt
+            and v.dtype == dt and dt in _TYPES):
+        raise w.ContractError("prompt attention operands: q [T, hq, 128], k and v [T, h, 128], fp16 or bf16, "
+                              "hq a multiple of h")
+    n = cu_seqlens.numel() - 1
+    if not (cu_seqlens.dtype == torch.int32 and cu_seqlens.ndim == 1 and n >= 0 and cu_seqlens.is_contiguous()):
+        raise w.ContractError("prompt attention cu_seqlens: contiguous int32 [seqs + 1]")
+    if not (q.is_cuda and k.device == dev and v.device == dev and cu_seqlens.device == dev):
+        raise w.ContractError("prompt attention operands on one CUDA device")
     (qt, qh, qc), (kt, kh, kc), (vt, vh, vc) = q.stride(), k.stride(), v.stride()
-    w.require(qc == kc == vc == 1 and not (qt | qh | kt | kh | vt | vh) & 7
-              and not (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15,
-              "prompt attention strides: contiguous channels, strides multiples of 8, 16-byte aligned")
-    T, hq = q.shape[0], q.shape[1]
+    qp, kp, vp = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    if not (qc == kc == vc == 1 and not (qt | qh | kt | kh | vt | vh) & 7 and not (qp | kp | vp) & 15):
+        raise w.ContractError("prompt attention strides: contiguous channels, strides multiples of 8, 16-byte aligned")
     if out is None:
-        out = torch.empty((T, hq, w.DIM), dtype=dt, device=dev)
+        out = torch.empty(qs, dtype=dt, device=dev)
+    elif not (out.shape == qs and out.dtype == dt and out.is_contiguous() and out.device == dev):
+        raise w.ContractError("prompt attention out: contiguous, of q's shape, dtype and device")
     if lse is None:
         lse = torch.empty((T, hq), dtype=torch.float32, device=dev)
-    w.require(out.shape == q.shape and out.dtype == dt and out.is_contiguous() and lse.shape == (T, hq)
-              and lse.dtype == torch.float32 and lse.is_contiguous() and out.device == dev and lse.device == dev,
-              "prompt attention outputs")
-    with torch.cuda.device(dev):
-        rc = L.load().nsnkv_prompt_attn(
-            T, cu_seqlens.numel() - 1, int(max_seqlen), hq, k.shape[1], L.DTYPE_CODE[dt], int(bool(causal)),
-            q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, cu_seqlens.data_ptr(), out.data_ptr(),
-            lse.data_ptr(), status.data_ptr() if status is not None else None,
-            torch.cuda.current_stream(dev).cuda_stream)
+    elif not (lse.shape == (T, hq) and lse.dtype == torch.float32 and lse.is_contiguous() and lse.device == dev):
+        raise w.ContractError("prompt attention lse: contiguous fp32 [T, hq] on q's device")
+    index = dev.index
+    rc = L.call_on(index, L.load().nsnkv_prompt_attn, T, n, int(max_seqlen), hq, h, _TYPES[dt], 1 if causal else 0, qp, qt,
+                   qh, kp, kt, kh, vp, vt, vh, cu_seqlens.data_ptr(), out.data_ptr(), lse.data_ptr(),
+                   None if status is None else status.data_ptr(), L.raw_stream(index))
     if rc:
         L.check(rc, "nsnkv_prompt_attn")
     return out, lse
