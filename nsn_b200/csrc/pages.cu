@@ -60,8 +60,14 @@ __global__ void __launch_bounds__(128) fork_kernel(const ForkArgs a) {
   const uint4 *from = reinterpret_cast<const uint4 *>(tail + s * a.tail_seq + head * a.tail_head);
   uint4 *to = reinterpret_cast<uint4 *>(tail + d * a.tail_seq + head * a.tail_head);
   const int n = min(max(a.tail_len[s], 0), kBlock) * (kDim * 2 / 16);
-#pragma unroll 8
-  for (int i = tid; i < n; i += 128) to[i] = from[i];
+  // at most 8 pieces per thread, all loaded before the first is stored
+  uint4 x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (tid + 128 * i < n) x[i] = from[tid + 128 * i];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (tid + 128 * i < n) to[tid + 128 * i] = x[i];
 }
 
 __global__ void __launch_bounds__(128) free_kernel(const ForkArgs a) {
@@ -154,53 +160,70 @@ __global__ void __launch_bounds__(kScan) reserve_kernel(int32_t *table, int64_t 
 
 // Compaction plan.  With L live pages (refs > 0, page 0 counted), the i-th live page at or
 // above L moves to the i-th free page below L, both in ascending order: the fewest moves that
-// bring the live pages to [0, L), and no destination is a source.  One CTA; each thread owns
-// a run of pages.
+// bring the live pages to [0, L), and no destination is a source.  One CTA: the counts are read
+// once, coalesced, into a bit per page (bits, before: one word per 32 pages), and ranks come
+// from a scan over the words.
 __global__ void __launch_bounds__(kScan) compact_plan_kernel(const int32_t *refs, int64_t pages, int32_t *refs_out,
                                                              int32_t *live_out, int32_t *src, int32_t *dst,
-                                                             int32_t *map, int32_t *moves) {
-  const int tid = threadIdx.x;
-  const int64_t per = (pages + kScan - 1) / kScan, p0 = min(tid * per, pages), p1 = min(p0 + per, pages);
-  __shared__ int below;  // live pages below L
+                                                             int32_t *map, int32_t *moves, uint32_t *bits,
+                                                             int32_t *before) {
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int words = static_cast<int>((pages + 31) / 32);
+#pragma unroll 4
+  for (int w = tid >> 5; w < words; w += kScan / 32) {
+    const int64_t p = static_cast<int64_t>(w) * 32 + lane;
+    const uint32_t m = __ballot_sync(0xffffffffu, p < pages && (p == 0 || refs[p] > 0));
+    if (lane == 0) bits[w] = m;
+  }
+  __syncthreads();
+  const int per = (words + kScan - 1) / kScan, w0 = min(tid * per, words), w1 = min(w0 + per, words);
   int n = 0;
-  for (int64_t p = p0; p < p1; ++p) n += p == 0 || refs[p] > 0;
+  for (int w = w0; w < w1; ++w) n += __popc(bits[w]);
   int live;
-  const int before = block_scan(n, live);
-  // live pages below L: every run counts its own part
-  int mine = 0;
-  for (int64_t p = p0; p < min(p1, static_cast<int64_t>(live)); ++p) mine += p == 0 || refs[p] > 0;
-  int low;
-  block_scan(mine, low);
+  int rank = block_scan(n, live);
+  __shared__ int below;  // live pages below L
+  if (tid == 0) below = live;
+  __syncthreads();
+  for (int w = w0; w < w1; ++w) {
+    before[w] = rank;
+    if (live >> 5 == w) below = rank + __popc(bits[w] & ((1u << (live & 31)) - 1u));
+    rank += __popc(bits[w]);
+  }
+  __syncthreads();
+  const int low = below;
   if (tid == 0) {
-    below = low;
     *live_out = live;
     *moves = live - low;
   }
-  __syncthreads();
-  int rank = before;
-  for (int64_t p = p0; p < p1; ++p) {
-    const bool used = p == 0 || refs[p] > 0;
+#pragma unroll 4
+  for (int w = tid >> 5; w < words; w += kScan / 32) {
+    const int p = w * 32 + lane;
+    const uint32_t m = bits[w];
+    const int r = before[w] + __popc(m & ((1u << lane) - 1u));
+    const bool used = m >> lane & 1;
+    if (p >= pages) continue;
     if (p >= live) {
       if (used)
-        src[rank - below] = static_cast<int32_t>(p);
+        src[r - low] = p;
       else
-        map[p] = static_cast<int32_t>(p);
+        map[p] = p;
     } else if (!used) {
-      dst[p - rank] = static_cast<int32_t>(p);
+      dst[p - r] = p;
     }
-    rank += used;
   }
   __syncthreads();
   // refs_out may be refs: counts move down first, then the pages at or above L are cleared
-  for (int i = tid; i < live - below; i += kScan) {
-    map[src[i]] = dst[i];
-    refs_out[dst[i]] = refs[src[i]];
+  for (int i = tid; i < live - low; i += kScan) {
+    const int s = src[i], d = dst[i];
+    map[s] = d;
+    refs_out[d] = refs[s];
   }
   __syncthreads();
-  for (int64_t p = p0; p < p1; ++p) {
+#pragma unroll 4
+  for (int64_t p = tid; p < pages; p += kScan) {
     if (p >= live)
       refs_out[p] = 0;
-    else if (p == 0 || refs[p] > 0)
+    else if (bits[p >> 5] >> (p & 31) & 1)
       refs_out[p] = refs[p];
   }
 }
@@ -218,8 +241,10 @@ struct MoveArgs {
   int32_t *status;
 };
 
-// Work item (move i, head j): the page's bytes of every array, 16 bytes per thread and load.
-constexpr int kMoveThreads = 128;
+// Work item (move i, head j): the page's bytes of every array in 16-byte pieces, kPieces per
+// thread and round, all loaded before the first is stored (a page is at most a few KB: one or
+// two rounds).  The next item's page numbers are read while an item is copied.
+constexpr int kMoveThreads = 128, kPieces = 4;
 __global__ void __launch_bounds__(kMoveThreads) move_kernel(const MoveArgs a) {
   const int tid = threadIdx.x;
   const int64_t gid = static_cast<int64_t>(blockIdx.x) * kMoveThreads + tid;
@@ -235,22 +260,37 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const MoveArgs a) {
       a.table_out[r * a.out_stride + c] = t;
     }
   }
-  const int32_t moves = a.count ? *a.count : a.max_count;
-  for (int64_t item = blockIdx.x; item < static_cast<int64_t>(moves) * a.h; item += gridDim.x) {
-    const int64_t i = item / a.h, j = item % a.h;
-    const int64_t s = a.src[i], d = a.dst[i];
+  const int64_t items = static_cast<int64_t>(a.count ? *a.count : a.max_count) * a.h;
+  int total = 0;
+  for (int x = 0; x < a.arrays; ++x) total += static_cast<int>(a.arr[x].bytes / 16);
+  int64_t item = blockIdx.x;
+  int32_t s = 0, d = 0;
+  if (item < items) s = a.src[item / a.h], d = a.dst[item / a.h];
+  while (item < items) {
+    const int64_t j = item % a.h, next = item + gridDim.x;
+    int32_t s_next = 0, d_next = 0;
+    if (next < items) s_next = a.src[next / a.h], d_next = a.dst[next / a.h];
     if (s < 0 || s >= a.pages || d < 0 || d >= a.pages) {
       if (tid == 0) set_status(a.status, NSNKV_ST_PAGE);
-      continue;
+    } else {
+      for (int u0 = 0; u0 < total; u0 += kMoveThreads * kPieces) {
+        uint4 v[kPieces], *to[kPieces];
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+          int u = u0 + i * kMoveThreads + tid, x = 0;
+          to[i] = nullptr;
+          if (u >= total) continue;
+          while (u >= a.arr[x].bytes / 16) u -= static_cast<int>(a.arr[x++].bytes / 16);
+          uint8_t *head = static_cast<uint8_t *>(a.arr[x].base) + j * a.arr[x].stride_head;
+          to[i] = reinterpret_cast<uint4 *>(head + d * a.arr[x].stride_page) + u;
+          v[i] = __ldcs(reinterpret_cast<const uint4 *>(head + s * a.arr[x].stride_page) + u);
+        }
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i)
+          if (to[i]) __stcs(to[i], v[i]);
+      }
     }
-    for (int x = 0; x < a.arrays; ++x) {
-      const nsnkv_page_array &p = a.arr[x];
-      const uint4 *from = reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(p.base) + j * p.stride_head + s * p.stride_page);
-      uint4 *to = reinterpret_cast<uint4 *>(static_cast<uint8_t *>(p.base) + j * p.stride_head + d * p.stride_page);
-      const int n = static_cast<int>(p.bytes / 16);
-#pragma unroll 4
-      for (int e = tid; e < n; e += kMoveThreads) to[e] = from[e];
-    }
+    item = next, s = s_next, d = d_next;
   }
 }
 
@@ -263,8 +303,8 @@ int check_arrays(int h, int64_t pages, int arrays, const nsnkv_page_array *arr) 
   return NSNKV_OK;
 }
 
-// CTAs of the move kernel: eight per SM keep enough loads in flight for the copy rate.
-constexpr int kMoveCtas = 148 * 8;
+// CTAs of the move kernel: twelve per SM, each with a page's loads in flight.
+constexpr int kMoveCtas = 148 * 12;
 
 }  // namespace
 }  // namespace nsnkv
@@ -347,7 +387,7 @@ int nsnkv_copy_pages(int h, int64_t pages, int arrays, const nsnkv_page_array *a
   return cudaGetLastError() == cudaSuccess ? NSNKV_OK : NSNKV_ERR_LAUNCH;
 }
 
-int64_t nsnkv_compact_pages_workspace_bytes(int64_t pages) { return pages > 0 ? (3 * pages + 1) * 4 : 0; }
+int64_t nsnkv_compact_pages_workspace_bytes(int64_t pages) { return pages > 0 ? (3 * pages + 2 + 2 * ((pages + 31) / 32)) * 4 : 0; }
 
 int nsnkv_compact_pages(int h, int64_t pages, int arrays, const nsnkv_page_array *arr, int64_t batch,
                         int32_t max_blocks, const int32_t *block_table, int64_t table_stride, int32_t *table_out,
@@ -361,7 +401,9 @@ int nsnkv_compact_pages(int h, int64_t pages, int arrays, const nsnkv_page_array
     return NSNKV_ERR_ARG;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int32_t *src = static_cast<int32_t *>(workspace), *dst = src + pages, *map = dst + pages, *moves = map + pages;
-  compact_plan_kernel<<<1, kScan, 0, st>>>(page_refs, pages, refs_out, live, src, dst, map, moves);
+  int32_t *bits = moves + 1, *before = bits + (pages + 31) / 32;
+  compact_plan_kernel<<<1, kScan, 0, st>>>(page_refs, pages, refs_out, live, src, dst, map, moves,
+                                           reinterpret_cast<uint32_t *>(bits), before);
   if (cudaGetLastError() != cudaSuccess) return NSNKV_ERR_LAUNCH;
   MoveArgs a{};
   for (int x = 0; x < arrays; ++x) a.arr[x] = arr[x];

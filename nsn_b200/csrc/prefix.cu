@@ -42,40 +42,61 @@ __device__ __forceinline__ int64_t row_at(const PrefixArgs &a, int64_t p) {
   return r >= 0 && r < a.rows ? r : -1;
 }
 
-// One warp per (query row, head): the chunks of its group and its own partial.
+// One warp per (query row, head): the chunks of its group and its own partial.  Lane c holds
+// chunk c's log-sum-exp; the chunks' rows are read four at a time.
 template <typename T>
 __global__ void __launch_bounds__(128) prefix_merge_kernel(const PrefixArgs a) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // launched while the chunk kernel runs
   const int lane = threadIdx.x & 31;
   const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
   if (item >= a.rows * a.hq) return;
-  const int64_t p = item / a.hq, head = item % a.hq;
+  const uint32_t hq = a.hq, p = static_cast<uint32_t>(item) / hq, head = static_cast<uint32_t>(item) - p * hq;
   const int64_t r = row_at(a, p);
   if (r < 0) return;
   int chunks = 0;
-  for (int g = 0; g < a.groups; ++g) {
-    int64_t begin, end;
-    group_rows(a, g, begin, end);
-    if (p >= begin && p < end) chunks = (group_pages(a, g) + a.chunk_pages - 1) / a.chunk_pages;
+  for (int g0 = 0; g0 < a.groups; g0 += 32) {
+    int64_t begin = 0, end = 0;
+    if (g0 + lane < a.groups) group_rows(a, g0 + lane, begin, end);
+    const bool in = p >= begin && p < end;
+    const int n = in ? (group_pages(a, g0 + lane) + a.chunk_pages - 1) / a.chunk_pages : 0;
+    chunks = max(chunks, __reduce_max_sync(0xffffffffu, n));
   }
   const int64_t at = r * a.hq + head, step = a.rows * a.hq;
-  float m = a.lse_part ? a.lse_part[at] * fm::kLog2e : -INFINITY;
-  const float own = m;
-  for (int c = 0; c < chunks; ++c) m = fmaxf(m, a.e_ws[c * step + at]);
-  const float base = m == -INFINITY ? 0.f : m;
-  float l = 0.f;
+  const float own = a.lse_part ? a.lse_part[at] * fm::kLog2e : -INFINITY;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto add = [&](float e, const float *row) {
-    const float w = fm::ex2(e - base);
-    if (e == -INFINITY) return;  // nothing seen: its row is not read
-    const float4 x = reinterpret_cast<const float4 *>(row)[lane];
-    l += w;
-    o.x += w * x.x;
-    o.y += w * x.y;
-    o.z += w * x.z;
-    o.w += w * x.w;
-  };
-  if (a.o_part) add(own, a.o_part + at * kDim);
-  for (int c = 0; c < chunks; ++c) add(a.e_ws[c * step + at], a.o_ws + (c * step + at) * kDim);
+  if (own != -INFINITY) o = reinterpret_cast<const float4 *>(a.o_part + at * kDim)[lane];  // else it is not read
+  float m = own, l = own == -INFINITY ? 0.f : 1.f;
+  for (int c0 = 0; c0 < chunks; c0 += 32) {
+    const float e = c0 + lane < chunks ? a.e_ws[(c0 + lane) * step + at] : -INFINITY;
+    float top = e;
+#pragma unroll
+    for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+    const float m_new = fmaxf(m, top), base = m_new == -INFINITY ? 0.f : m_new;
+    const float w = e == -INFINITY ? 0.f : fm::ex2(e - base), c = m == -INFINITY ? 0.f : fm::ex2(m - base);
+    float sum = w;
+#pragma unroll
+    for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    l = l * c + sum;
+    o.x *= c, o.y *= c, o.z *= c, o.w *= c;
+    m = m_new;
+    const int n = min(32, chunks - c0);
+    for (int i = 0; i < n; i += 4) {
+      float4 x[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (i + k < n) x[k] = reinterpret_cast<const float4 *>(a.o_ws + ((c0 + i + k) * step + at) * kDim)[lane];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float wk = __shfl_sync(0xffffffffu, w, (i + k) & 31);
+        if (i + k < n && wk != 0.f) {  // 0: the chunk holds nothing for the row (NaN passes)
+          o.x += wk * x[k].x;
+          o.y += wk * x[k].y;
+          o.z += wk * x[k].z;
+          o.w += wk * x[k].w;
+        }
+      }
+    }
+  }
   const float inv = m == -INFINITY ? 0.f : __fdiv_rn(1.f, l);
   const uint2 w = make_uint2(fm::round_pair<T>(o.x * inv, o.y * inv), fm::round_pair<T>(o.z * inv, o.w * inv));
   reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + at * kDim)[lane] = w;
@@ -115,8 +136,16 @@ int launch(const PrefixArgs &a, int64_t chunks, cudaStream_t st) {
     kern<<<dim3(static_cast<unsigned>(chunks), a.h, a.groups * a.row_tiles), xtc::kThreads, smem, st>>>(x);
     if (cudaGetLastError() != cudaSuccess) return NSNKV_ERR_LAUNCH;
   }
-  prefix_merge_kernel<T><<<static_cast<unsigned>((a.rows * a.hq + 3) / 4), 128, 0, st>>>(a);
-  return cudaGetLastError() == cudaSuccess ? NSNKV_OK : NSNKV_ERR_LAUNCH;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>((a.rows * a.hq + 3) / 4));
+  cfg.blockDim = dim3(128);
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = chunks > 0 ? 1 : 0;  // only behind the chunk kernel, which announces it
+  return cudaLaunchKernelEx(&cfg, prefix_merge_kernel<T>, a) == cudaSuccess ? NSNKV_OK : NSNKV_ERR_LAUNCH;
 }
 
 }  // namespace
@@ -152,7 +181,7 @@ int nsnkv_prefix_attn(int64_t rows, int32_t groups, int64_t max_rows, int hq, in
   if (nsnkv_prefix_attn_workspace_bytes(rows, groups, hq, h, max_pages) > workspace_bytes ||
       (max_pages > 0 && (!workspace || !aligned16(workspace))))
     return NSNKV_ERR_ARG;
-  if (rows * hq > (int64_t{1} << 32) || groups > 4096) return NSNKV_ERR_TOO_LARGE;
+  if (rows * hq > INT32_MAX || groups > 4096) return NSNKV_ERR_TOO_LARGE;
   const int G = hq / h;
   const int chunk = max_pages ? chunk_pages_for(rows, groups, G, h, max_pages) : 1;
   const int64_t chunks = max_pages ? max_chunks(max_pages, chunk) : 0;

@@ -138,8 +138,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
     begin = min(max(static_cast<int64_t>(a.row_offsets[group]), int64_t{0}), a.rows);
     end = min(max(static_cast<int64_t>(a.row_offsets[group + 1]), begin), a.rows);
   }
-  const int64_t nrows = (end - begin) * G;
-  if (nloc <= 0 || (blockIdx.z % a.pairs) * int64_t{2 * kM} >= nrows) return;
+  const int nrows = static_cast<int>(end - begin) * G;  // rows * hq fits an int
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge may take its place behind this grid
+  if (nloc <= 0 || (blockIdx.z % a.pairs) * 2 * kM >= nrows) return;
 
   if (warp == 16) {
     tc::tmem_alloc(&S.tmem, 512);
@@ -167,7 +168,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
   __syncthreads();
   tc::fence_after();
   const uint32_t tmem = S.tmem;
-  const uint32_t kR = (blockIdx.z % a.pairs) * int64_t{2 * kM} + kM < nrows ? kRaw<BITS> : kRawWide<BITS>;
+  const uint32_t kR = static_cast<int>(blockIdx.z % a.pairs) * 2 * kM + kM < nrows ? kRaw<BITS> : kRawWide<BITS>;
   auto raw = [&](uint32_t slot) {
     return slot < kRaw<BITS> ? S.raw[slot] : S.q[1] + (slot - kRaw<BITS>) * R::kBytes;
   };
@@ -176,27 +177,27 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
   // Ring positions and parities run on from one to the next.
   uint32_t blocks = 0, pair_n = 0;  // blocks and pairs taken so far
   uint32_t taken[2] = {0, 0};       // blocks that each softmax team has taken so far
-  for (int64_t row0 = (blockIdx.z % a.pairs) * int64_t{2 * kM}; row0 < nrows;
-       row0 += static_cast<int64_t>(a.pairs) * 2 * kM, blocks += nloc, ++pair_n) {
+  for (int row0 = (blockIdx.z % a.pairs) * 2 * kM; row0 < nrows;
+       row0 += a.pairs * 2 * kM, blocks += nloc, ++pair_n) {
     const int tiles = row0 + kM < nrows ? 2 : 1;  // row tiles of this pair
     const bool split = tiles == 1;                // the teams share one tile
     const int team_blocks[2] = {split ? (nloc + 1) / 2 : nloc, split ? nloc / 2 : nloc};
     if (warp < 8) {  // ---- Q, softmax, output
       const int t = warp >> 2;
-      const int64_t first = row0 + (split ? 0 : t * kM);
+      const int first = row0 + (split ? 0 : t * kM);
       if (t < tiles) {
         // Q of the tile into its swizzled place: 16 threads per row
         int bad = 0;
-#pragma unroll 4
+#pragma unroll 8
         for (int i = 0; i < 16; ++i) {
           const int r = i * 8 + ((tid & 127) >> 4), c = tid & 15;
-          const int64_t rr_ = first + r;
           uint4 x = make_uint4(0u, 0u, 0u, 0u);
-          if (rr_ < nrows) {
-            const int64_t pos = begin + rr_ / G;
-            const int64_t qr = a.row_index ? a.row_index[pos] : pos;
+          if (first + r < nrows) {
+            const uint32_t p = static_cast<uint32_t>(first + r) / static_cast<uint32_t>(G);
+            const int64_t pos = begin + p, qr = a.row_index ? a.row_index[pos] : pos;
             if (qr >= 0 && qr < a.rows)
-              x = reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + (qr * a.hq + head * G + rr_ % G) * kDim)[c];
+              x = reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) +
+                                                  (qr * a.hq + head * G + (first + r - p * G)) * kDim)[c];
           }
           const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
@@ -293,14 +294,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
         }
         if (team_blocks[t]) tc::spin(&S.o_done[t], (taken[t] + team_blocks[t] - 1) & 1, &S.failed, a.status);
         tc::fence_after();
-        const int64_t r = first + (tid & 127);
+        const int r = first + (tid & 127), pr = r / G;
         int64_t qr = -1;
-        if (r < nrows) {
-          const int64_t pos = begin + r / G;
-          qr = a.row_index ? a.row_index[pos] : pos;
-        }
+        if (r < nrows) qr = a.row_index ? a.row_index[begin + pr] : begin + pr;
         const bool mine = qr >= 0 && qr < a.rows;
-        const int64_t at = (blockIdx.x * a.rows + qr) * a.hq + head * G + r % G;
+        const int64_t at = (blockIdx.x * a.rows + qr) * a.hq + head * G + (r - pr * G);
         float inv = m == -INFINITY ? 0.f : __fdiv_rn(1.f, l), e2 = m == -INFINITY ? -INFINITY : m + log2f(l);
         // Team 1's half of a shared tile goes through shared memory (Q's place: every S is done,
         // each team having seen its last P.V), column by column of all rows.
@@ -522,7 +520,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
     }
     taken[0] += team_blocks[0], taken[1] += team_blocks[1];
     // The next pair reuses O, the Q tiles and, where a row tile had no rows, untouched barriers.
-    if (row0 + static_cast<int64_t>(a.pairs) * 2 * kM < nrows) {
+    if (row0 + a.pairs * 2 * kM < nrows) {
       tc::fence_before();
       __syncthreads();
       tc::fence_after();

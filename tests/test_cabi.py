@@ -189,5 +189,5 @@ def test_shared_prompt_operators_refuse_on_the_host():
     arr[0].bytes = 60
     assert lib.nsnkv_copy_pages(2, 8, 1, arr, 1, P, P, N, N) == _lib.ERR_ARG
     arr[0].bytes = 64
-    assert lib.nsnkv_compact_pages_workspace_bytes(8) == 100
-    assert lib.nsnkv_compact_pages(2, 8, 1, arr, 2, 4, P, 4, P, 4, P, P, P, P, 99, N, N) == _lib.ERR_ARG
+    assert lib.nsnkv_compact_pages_workspace_bytes(8) >= 100
+    assert lib.nsnkv_compact_pages(2, 8, 1, arr, 2, 4, P, 4, P, 4, P, P, P, P, 15, N, N) == _lib.ERR_ARG
