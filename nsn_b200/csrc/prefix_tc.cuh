@@ -32,6 +32,7 @@ constexpr int kThreads = 640;
 // the next raise, and p of the largest, 2^-6, leaves fp16's 2^-24 far below its rounding.
 constexpr float kHeadroom = 6.f;
 constexpr int kStages = 4;  // restored blocks held
+constexpr int kStageRow = kDim * 4 + 16;  // a staged output row (bytes)
 constexpr int kRowsBytes = kBlock * kDim * 2;  // K or V of one block
 
 // Records in flight: their own slots, and with one row tile the slots that fit the other tile's Q.
@@ -39,7 +40,7 @@ template <int BITS> constexpr int kRaw = BITS == 3 ? 3 : 2;
 template <int BITS> constexpr int kRawWide = kRaw<BITS> + kM * kDim * 2 / rr::Rec<BITS>::kBytes;
 
 template <int BITS>
-struct Smem {
+struct Smem {  // q and kv also stage two tiles of output rows, or one behind the other team's half
   uint8_t q[2][kM * kDim * 2];
   uint8_t kv[kStages][2][kRowsBytes];  // each [2 halves of 64 channels][64 tokens][128 B swizzled]
   uint8_t raw[kRaw<BITS>][rr::Rec<BITS>::kBytes];
@@ -186,27 +187,35 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
       const int t = warp >> 2;
       const int first = row0 + (split ? 0 : t * kM);
       if (t < tiles) {
-        // Q of the tile into its swizzled place: 16 threads per row
-        int bad = 0;
-#pragma unroll 8
-        for (int i = 0; i < 16; ++i) {
-          const int r = i * 8 + ((tid & 127) >> 4), c = tid & 15;
-          uint4 x = make_uint4(0u, 0u, 0u, 0u);
-          if (first + r < nrows) {
-            const uint32_t p = static_cast<uint32_t>(first + r) / static_cast<uint32_t>(G);
-            const int64_t pos = begin + p, qr = a.row_index ? a.row_index[pos] : pos;
-            if (qr >= 0 && qr < a.rows)
-              x = reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) +
-                                                  (qr * a.hq + head * G + (first + r - p * G)) * kDim)[c];
-          }
-          const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        // Q of the tile into its swizzled place: 16 threads per row, eight rows' pieces on their
+        // way at a time (a rolled loop: this code runs once, and cold code costs its fetch).
+        constexpr uint32_t kExp = Elem<T>::kBf16 ? 0x7F807F80u : 0x7C007C00u, kOne = Elem<T>::kBf16 ? 0x00800080u : 0x04000400u;
+        uint32_t bad = 0;
+        const int c = tid & 15;
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          const int r0 = 64 * h + ((tid & 127) >> 4);
+          uint4 x[8];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 f = Elem<T>::to_f2(w[e]);
-            bad |= !isfinite(f.x) || !isfinite(f.y);
+          for (int i = 0; i < 8; ++i) {
+            const int r = first + r0 + 8 * i, p = r / G;
+            x[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (r < nrows) {
+              const int64_t qr = a.row_index ? __ldg(a.row_index + begin + p) : begin + p;
+              if (qr >= 0 && qr < a.rows)
+                x[i] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) +
+                                                             (qr * a.hq + head * G + (r - p * G)) * kDim) + c);
+            }
           }
-          *reinterpret_cast<uint4 *>(S.q[t] + (c >> 3) * (kM * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = x;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int r = r0 + 8 * i;
+            // an exponent of all ones (NaN, infinity) carries into the sign's place
+            bad |= ((x[i].x & kExp) + kOne) | ((x[i].y & kExp) + kOne) | ((x[i].z & kExp) + kOne) | ((x[i].w & kExp) + kOne);
+            *reinterpret_cast<uint4 *>(S.q[t] + (c >> 3) * (kM * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = x[i];
+          }
         }
+        bad &= 0x80008000u;
         if (bad) set_status(a.status, NSNKV_ST_INPUT_NONFINITE);
         tc::fence_async();
         __syncwarp();
@@ -300,11 +309,14 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
         const bool mine = qr >= 0 && qr < a.rows;
         const int64_t at = (blockIdx.x * a.rows + qr) * a.hq + head * G + (r - pr * G);
         float inv = m == -INFINITY ? 0.f : __fdiv_rn(1.f, l), e2 = m == -INFINITY ? -INFINITY : m + log2f(l);
-        // Team 1's half of a shared tile goes through shared memory (Q's place: every S is done,
-        // each team having seen its last P.V), column by column of all rows.
+        // Both teams have seen their last P.V: every MMA is done, and Q and the ring are free.  Team
+        // 1's half of a shared tile goes to team 0 through them, column by column of all rows;
+        // finished rows are staged there and leave in one bulk copy each (rows 16 bytes apart
+        // from a multiple of 128, so that a warp's writes fall into different banks).
         float *other = reinterpret_cast<float *>(S.q) + (tid & 127);
+        uint8_t *stage = S.q[0] + (split ? 1 : t) * (kM * kStageRow) + (tid & 127) * kStageRow;
         float w = 0.f;
-        if (split) tc::bar_named(3, 256);
+        tc::bar_named(3, 256);
         if (split && t == 0) {
           tc::bar_named(4, 256);
           const float e1 = S.e_other[tid & 127], top = fmaxf(e2, e1), b0 = top == -INFINITY ? 0.f : top;
@@ -332,10 +344,18 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
 #pragma unroll
               for (int e = 0; e < 32; ++e) o[e] = fmaf(w, other[(32 * i + e) * kM], o[e]);
             }
-            if (mine)
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                tc::store32(a.o_ws + at * kDim + 32 * i + 8 * e, reinterpret_cast<uint32_t *>(o) + 8 * e);
+            for (int e = 0; e < 8; ++e)
+              *reinterpret_cast<float4 *>(stage + 128 * i + 16 * e) =
+                  make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          }
+          if (mine && !(split && t == 1)) {
+            tc::fence_async();
+            asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], 512;" ::"l"(a.o_ws + at * kDim),
+                         "r"(tc::saddr(stage))
+                         : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
           }
         }
         tc::fence_before();
