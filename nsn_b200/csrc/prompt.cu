@@ -149,14 +149,7 @@ int launch_rows(const PromptArgs &a, int64_t longest, cudaStream_t st) {
 // Tensor map of x [tokens][heads][128] with element strides: boxes of 64 channels of one
 // head and 128 tokens, 128-byte swizzle.
 bool make_map(CUtensorMap *map, const void *base, int dtype, int64_t tokens, int heads, int64_t tok, int64_t head) {
-  static const auto encode = [] {
-    void *fn = nullptr;
-    cudaDriverEntryPointQueryResult got;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &got) != cudaSuccess ||
-        got != cudaDriverEntryPointSuccess)
-      fn = nullptr;
-    return reinterpret_cast<decltype(&cuTensorMapEncodeTiled)>(fn);
-  }();
+  const auto encode = tc::encoder();
   if (!encode) return false;
   const cuuint64_t dims[3] = {kDim, static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(tokens)};
   // the stride of a dimension of one element is never used
