@@ -8,6 +8,10 @@ Modules mirror the reference's operator surface:
   kernel      restore_v / launch / pipeline (fused packed-KV decode attention)
   paged       PagedKVCache (batched paged cache: append + attend + seal)
   splitkv     sequence-split decode across GPUs with a log-sum-exp merge
+  prompt      attention over whole packed prompts (causal, grouped heads, ragged lengths)
+  prefix      attention over a sealed prefix that many rows share, merged with their own part
+  pages       fork / free / reserve / copy / compact of a page pool
+  shared      SharedPagedKVCache and SharedPromptDecoder: sequences that share pages
 All compute runs in libnsnkv.so (include/nsnkv.h); there is no CPU fallback.
 """
 from . import primitives  # noqa: F401

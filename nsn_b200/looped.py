@@ -105,8 +105,7 @@ class PagedLoopedDecoder:
         self.dtype = model.embed.weight.dtype
         self.max_blocks = -(-max_tokens // 64) + 1  # a spare page: a full tail always finds one
         n_slots = model.loops * len(model.layers)
-        self.caches = [PagedKVCache(batch, self.h, self.max_blocks, bits=3, dtype=self.dtype, device=self.device,
-                                    hq=self.hq, restore_rounding=restore_rounding) for _ in range(n_slots)]
+        self.caches = [self._new_cache(restore_rounding) for _ in range(n_slots)]
         # the decode step's fused weights: q|k|v and gate|up concatenated (copies; the model's
         # own modules keep theirs for the prefill)
         self.fused = []
@@ -122,6 +121,10 @@ class PagedLoopedDecoder:
         self._ids = torch.zeros(batch, dtype=torch.long, device=self.device)
         self._pos = torch.zeros((1, 1), dtype=torch.long, device=self.device)
         self._logits = None
+
+    def _new_cache(self, restore_rounding):
+        return PagedKVCache(self.batch, self.h, self.max_blocks, bits=3, dtype=self.dtype, device=self.device,
+                            hq=self.hq, restore_rounding=restore_rounding)
 
     # ------------------------------------------------------------ prefill: the model's own modules
     def _prefill_layer(self, layer, h, cos, sin, cache):

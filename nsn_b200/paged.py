@@ -171,8 +171,12 @@ ROUNDING_MODES = ("k", "kv", "exact")
 
 class PagedKVCache:
     def __init__(self, batch: int, h: int, max_blocks: int, bits: int = 3, dtype=torch.float16, device="cuda",
-                 hq: int | None = None, bridge_rounding: bool = False, restore_rounding: str | None = None):
-        """How attention treats the restored rows (``restore_rounding``):
+                 hq: int | None = None, bridge_rounding: bool = False, restore_rounding: str | None = None,
+                 pages: int | None = None):
+        """``pages``: the pool's pages when the block table is filled page by page
+        (shared.SharedPagedKVCache); by default sequence b owns max_blocks pages of its own.
+
+        How attention treats the restored rows (``restore_rounding``):
 
         ``"k"`` (default): K rows rounded to the cache dtype exactly as the reference
             bridge (restore_group(g, dtype) + SDPA) rounds them, V applied as the exact fp32
@@ -202,7 +206,7 @@ class PagedKVCache:
         w.require(self.device.type == "cuda", "paged cache device (CUDA only)")
         if self.device.index is None:  # "cuda": the current device, named, so tensors compare equal
             self.device = torch.device("cuda", torch.cuda.current_device())
-        self.pages = batch * max_blocks
+        self.pages = batch * max_blocks if pages is None else pages
         cb = w.code_bytes(bits)
         dev = self.device
 
@@ -219,7 +223,9 @@ class PagedKVCache:
             self.blk_bytes = self.records.shape[-1]
         else:
             self.k_pool, self.v_pool = pool(), pool()
-        self.block_table = torch.arange(self.pages, dtype=torch.int32, device=dev).reshape(batch, max_blocks)
+        self.block_table = torch.zeros((batch, max_blocks), dtype=torch.int32, device=dev)
+        if pages is None:
+            self.block_table.copy_(torch.arange(self.pages, dtype=torch.int32, device=dev).reshape(batch, max_blocks))
         self.n_blocks = torch.zeros(batch, dtype=torch.int32, device=dev)
         self.tail_len = torch.zeros(batch, dtype=torch.int32, device=dev)
         # host copies of n_blocks / tail_len, kept without reading the device: every change

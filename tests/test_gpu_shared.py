@@ -1,0 +1,142 @@
+"""The shared cache and the decoder over it, against caches that share nothing."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def rows(n, h, seed, dtype=torch.float16):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return [torch.randn((h, n, 128), generator=g, device="cuda").to(dtype) for _ in range(2)]
+
+
+def token(batch, hq, h, seed, dtype=torch.float16):
+    g = torch.Generator(device="cuda").manual_seed(1000 + seed)
+    return [torch.randn((batch, x, 128), generator=g, device="cuda").to(dtype) for x in (hq, h, h)]
+
+
+def refs_hold(c):
+    want = np.bincount(c.block_table.cpu().numpy().reshape(-1), minlength=c.pages)
+    want[0] = 1
+    assert np.array_equal(c.page_refs.cpu().numpy(), want)
+    assert np.array_equal(c.n_blocks.cpu().numpy(), c.host_blocks) and np.array_equal(c.tail_len.cpu().numpy(),
+                                                                                      c.host_tail)
+
+
+@pytest.mark.parametrize("bits,dtype,hq", [(3, torch.float16, 8), (3, torch.bfloat16, 16), (5, torch.float16, 4)])
+@pytest.mark.parametrize("prompt", [64, 64 * 5 + 17, 63])
+def test_forked_sequences_decode_like_separate_ones(bits, dtype, hq, prompt):
+    """Plain and shared steps over forks against an ordinary cache holding the prompt per
+    sequence, across seals.  Both round K; V is fp32-restored there and rounded to dtype in the
+    shared prefix, so outputs differ by V's, p's and the outputs' roundings: 4 units of dtype."""
+    from nsn_b200.paged import PagedKVCache
+    from nsn_b200.shared import SharedPagedKVCache
+    batch, h, steps = 5, 2, 70
+    k, v = rows(prompt, h, 1, dtype)
+    plain = PagedKVCache(batch, h, 9, bits=bits, dtype=dtype, hq=hq)
+    for b in range(batch):
+        plain.prefill(b, k, v)
+    shared = SharedPagedKVCache(batch, h, 9, 8 + 3 * batch, bits=bits, dtype=dtype, hq=hq)
+    shared.prefill(2, k, v)
+    shared.fork(2, [0, 1, 3, 4])
+    refs_hold(shared)
+    plan = shared.share([[2, 0, 1, 4]])  # sequence 3 outside the group
+    unit = 2.0 ** (-10 if dtype == torch.float16 else -7)
+    for i in range(steps):
+        q, kn, vn = token(batch, hq, h, i, dtype)
+        want = plain.step(q, kn, vn).float()
+        got = (shared.step_shared(plan, q, kn, vn) if i % 3 else shared.step(q, kn, vn)).float()
+        if not i % 3:
+            plan.refresh(shared)
+        assert float((got - want).abs().max()) <= 4 * unit * max(1.0, float(want.abs().max())), i
+    shared.check()
+    refs_hold(shared)
+    for b in range(batch):
+        for x, y in zip(plain.export_groups(b), shared.export_groups(b)):
+            if isinstance(x, dict):
+                assert torch.equal(x["codes"], y["codes"]) and all(torch.equal(s, t) for s, t in zip(x["metas"],
+                                                                                                     y["metas"]))
+            else:
+                assert (x is None and y is None) or torch.equal(x, y)
+
+
+def test_free_compact_and_reuse():
+    from nsn_b200.shared import SharedPagedKVCache
+    c = SharedPagedKVCache(4, 2, 12, 40, hq=4)
+    for b in range(3):
+        c.prefill(b, *rows(64 * (3 + 2 * b) + 9, 2, b))
+    before = [c.to_bytes(b) for b in range(3)]
+    c.fork(1, 3)
+    c.free([0])
+    refs_hold(c)
+    live = c.compact()
+    refs_hold(c)
+    held = int((c.page_refs > 0).sum())
+    assert int(live) == held and int(c.block_table.max()) < held
+    assert [c.to_bytes(b) for b in (1, 2, 3)] == [before[1], before[2], before[1]]
+    c.prefill(0, *rows(64 * 3 + 9, 2, 0))
+    assert c.to_bytes(0) == before[0] and c.to_bytes(2) == before[2]
+    refs_hold(c)
+    c.load_bytes(3, before[2])
+    assert c.to_bytes(3) == before[2]
+    refs_hold(c)
+    c.check()
+
+
+def test_pool_exhaustion_is_reported():
+    from nsn_b200 import ContractError
+    from nsn_b200.shared import SharedPagedKVCache
+    c = SharedPagedKVCache(2, 1, 8, 6, hq=2)
+    c.prefill(0, *rows(64 * 3, 1, 0))
+    c.check()
+    c.prefill(1, *rows(64 * 3, 1, 1))
+    with pytest.raises(ContractError):
+        c.check()
+
+
+def test_refusals():
+    from nsn_b200 import ContractError
+    from nsn_b200.shared import SharedPagedKVCache
+    c = SharedPagedKVCache(3, 1, 4, 20, hq=2)
+    c.prefill(0, *rows(70, 1, 0))
+    for bad in (lambda: c.fork(0, [0]), lambda: c.fork(0, [1, 1]), lambda: c.fork([0, 1], [1, 2]), lambda: c.fork(0, 3),
+                lambda: c.share([[0, 1], [1, 2]]), lambda: c.share([[]]), lambda: c.extend(0, *rows(5, 1, 0)),
+                lambda: c.prefill(1, *rows(64 * 5, 1, 0)), lambda: SharedPagedKVCache(3, 1, 4, 3, hq=2),
+                lambda: SharedPagedKVCache(3, 1, 4, 20, bits=4, hq=2)):
+        with pytest.raises(ContractError):
+            bad()
+
+
+@pytest.mark.parametrize("prompt", [200, 256])
+def test_shared_prompt_decoder(prompt):
+    """Teacher-forced logits of samples of one prompt: the shared decoder against the batched
+    decoder given the prompt per sequence, eager and replayed."""
+    from transformers import LlamaConfig
+    from nsn_b200 import adapter
+    from nsn_b200.looped import PagedLoopedDecoder
+    from nsn_b200.shared import SharedPromptDecoder
+    torch.manual_seed(0)
+    cfg = LlamaConfig(hidden_size=256, num_attention_heads=2, num_key_value_heads=1, head_dim=128, num_hidden_layers=2,
+                      intermediate_size=512, vocab_size=320, rope_theta=10000.0)
+    model = adapter.LoopedDecoder(cfg, loops=2).cuda().half().eval()
+    batch = 3
+    ids = torch.randint(0, 320, (prompt,), device="cuda")
+    nxt = torch.randint(0, 320, (80, batch), device="cuda")
+    a = PagedLoopedDecoder(model, batch, prompt + 100)
+    b = SharedPromptDecoder(model, batch, prompt + 100)
+    la, lb = a.prefill(ids[None].expand(batch, -1)), b.prefill(ids)
+    scale = float(la.abs().max())
+    # two attention roundings per layer evaluation (4 evaluations) of fp16 activations, with margin
+    tol = 4 * 8 * 2.0 ** -10 * scale
+    assert float((la[0] - lb).abs().max()) <= tol
+    for i in range(75):
+        if i == 4:
+            b.capture()
+        x, y = a.step(nxt[i]), (b.replay(nxt[i]) if i >= 4 else b.step(nxt[i]))
+        assert float((x - y).abs().max()) <= tol, i
+    b.sync_counters()
+    b.release()
+    b.check()
+    for c in b.caches:
+        refs_hold(c)
