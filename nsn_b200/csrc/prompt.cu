@@ -203,7 +203,10 @@ extern "C" int nsnkv_prompt_attn(int64_t tokens, int32_t seqs, int64_t longest, 
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (longest > tokens) longest = tokens;
   if (tokens > INT32_MAX || (tokens / 256 + seqs) * hq > INT32_MAX) return NSNKV_ERR_TOO_LARGE;
-  if (longest >= 256 && (reinterpret_cast<uintptr_t>(out) & 31) == 0)
+  // The tensor-core kernel from 65 rows on: 16 sequences of 64 tokens, GQA 32:8, take 18.3 us here and
+  // 19.9 us there, of 128 tokens 33.0 and 21.8 us, of 256 tokens 72.6 and 36.2 us.  Its stores are
+  // 32 bytes wide.
+  if (longest > 64 && (reinterpret_cast<uintptr_t>(out) & 31) == 0)
     return dtype == NSNKV_F16 ? launch_tc<__half>(a, dtype, st) : launch_tc<__nv_bfloat16>(a, dtype, st);
   return dtype == NSNKV_F16 ? launch_rows<__half>(a, longest, st) : launch_rows<__nv_bfloat16>(a, longest, st);
 }

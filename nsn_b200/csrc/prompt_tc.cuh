@@ -30,8 +30,6 @@ constexpr int kStages = 5;
 constexpr int kTileBytes = kN * kDim * 2;
 constexpr int kThreads = 384;
 constexpr float kRaise = 8.f;
-constexpr int kLag = 3, kAhead = 4;
-constexpr int kPoly = 0, kPolyEvery = 4;  // kPoly of kPolyEvery pairs take ex2_poly
 
 constexpr int kItems = 4;  // items laid out ahead
 
@@ -60,26 +58,6 @@ struct Args {
 struct Maps {
   CUtensorMap q, k, v;
 };
-
-// 2^x of a pair on the FMA pipes: x = n + f with n the nearest integer and |f| <= 1/2, 2^f by a
-// degree-4 minimax polynomial (relative error 2.6e-6, least squares iterated to the equal
-// ripple), n added to the exponent.  x below -126 gives 2^-126.  The special function unit takes
-// 8 cycles per warp for an exponential, 2048 for the two row tiles of a K / V tile: as long as
-// the tile's MMAs, so a part of the exponentials is done here.
-__device__ __forceinline__ float2 ex2_poly(float2 x) {
-  x.x = fmaxf(x.x, -126.f);
-  x.y = fmaxf(x.y, -126.f);
-  const float2 big = make_float2(12582912.f, 12582912.f);  // 1.5 * 2^23: the sum's low bits hold n
-  const float2 t = tc::add2(x, big);
-  const float2 f = tc::fma2(tc::add2(t, make_float2(-12582912.f, -12582912.f)), make_float2(-1.f, -1.f), x);
-  auto c2 = [](float c) { return make_float2(c, c); };
-  float2 p = tc::fma2(c2(0.009570101276040077f), f, c2(0.05591785907745361f));
-  p = tc::fma2(p, f, c2(0.240247443318367f));
-  p = tc::fma2(p, f, c2(0.6931217908859253f));
-  p = tc::fma2(p, f, c2(0.9999992847442627f));
-  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
-                     __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
-}
 
 // One softmax warpgroup over its row tile.  P is announced in two halves of 64 tokens: the P.V
 // MMAs of the first run while the second is computed.
@@ -149,22 +127,15 @@ __device__ __forceinline__ void softmax_tiles(const Args &a, Smem &S, int t, int
 #pragma unroll 1
     for (int h = 0; h < 2; ++h) {
       load(h);
-      // Pair e's exponentials issue kLag pairs before its sum and conversion, so that the warp
-      // does not wait for the special function unit's latency.
-      float2 *x = reinterpret_cast<float2 *>(s);
-      uint32_t p[16];
+      uint32_t p[32];
 #pragma unroll
-      for (int e = 0; e < kAhead; ++e) x[e] = tc::fma2(x[e], sc2, nb2);
-#pragma unroll
-      for (int e = 0; e < 32 + kLag; ++e) {
-        if (e + kAhead < 32) x[e + kAhead] = tc::fma2(x[e + kAhead], sc2, nb2);
-        if (e < 32) x[e] = e % kPolyEvery < kPoly ? ex2_poly(x[e]) : make_float2(fm::ex2(x[e].x), fm::ex2(x[e].y));
-        if (e < kLag) continue;
-        const int d = e - kLag;
-        if (d & 1) l2 = tc::add2(l2, x[d]); else l = tc::add2(l, x[d]);
-        p[d & 15] = fm::round_pair<T>(x[d].x, x[d].y);
-        if ((d & 15) == 15) tc::st16(s_at + 32 * h + (d & ~15), p);
+      for (int e = 0; e < 32; ++e) {
+        const float2 x = tc::fma2(make_float2(s[2 * e], s[2 * e + 1]), sc2, nb2);
+        const float2 y = make_float2(fm::ex2(x.x), fm::ex2(x.y));
+        if (e & 1) l2 = tc::add2(l2, y); else l = tc::add2(l, y);
+        p[e] = fm::round_pair<T>(y.x, y.y);
       }
+      tc::st32(s_at + 32 * h, p);
       tc::wait_st();
       tc::fence_before();
       __syncwarp();
