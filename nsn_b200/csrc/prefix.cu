@@ -109,81 +109,42 @@ __global__ void __launch_bounds__(128) prefix_merge_kernel(const PrefixArgs a) {
 constexpr int kSms = 148;
 constexpr int kPairRows = 2 * xtc::kM;
 
-// How a call is split.
-struct Split {
-  int chunk_pages = 1;
-  int64_t chunks = 0;  // at most, of a group
-  bool rows = false;   // blocks restored ahead, into the workspace
-};
-// One CTA per SM and (chunk, head, pair of row tiles): a CTA costs about its pages plus five for
-// its start, its partial rows and their merge.  A block restored in place costs a pair of row tiles
-// about 2700 cycles of its SM, one restored ahead about 1700 and 1500 once for all pairs (the
-// write and the reads of its rows stay in L2 up to some 100 MB): ahead from four pairs per group
-// on (1501 rows of three groups, GQA 32:8: 261 us in place).
-Split split_for(int64_t rows, int groups, int G, int h, int32_t max_pages) {
-  Split s;
-  if (max_pages <= 0) return s;
-  const int64_t pairs = (rows * G + kPairRows - 1) / kPairRows, units = (pairs + groups - 1) * h;
+// Pages per chunk.  The kernel runs one CTA per SM and (chunk, head, pair of row tiles); a CTA
+// costs about its pages plus five for its start, its partial rows and their merge.
+int chunk_pages_for(int64_t rows, int groups, int G, int h, int32_t max_pages) {
+  const int64_t units = ((rows * G + kPairRows - 1) / kPairRows + groups - 1) * h;
   int64_t best = max_pages, best_cost = INT64_MAX;
   for (int64_t chunks = 1; chunks <= kSms && chunks <= max_pages; ++chunks) {
     const int64_t per = (max_pages + chunks - 1) / chunks, waves = (units * ((max_pages + per - 1) / per) + kSms - 1) / kSms;
     const int64_t cost = waves * (per + 5);
     if (cost < best_cost) best = per, best_cost = cost;
   }
-  s.chunk_pages = static_cast<int>(best < 1 ? 1 : best);
-  s.chunks = (max_pages + s.chunk_pages - 1) / s.chunk_pages;
-  const int64_t blocks = static_cast<int64_t>(groups) * h * max_pages;
-  s.rows = pairs >= 4 * groups && blocks * 2 * kBlock <= INT32_MAX && blocks * 2 * xtc::kRowsBytes <= (int64_t{2} << 30);
-  return s;
+  return static_cast<int>(best < 1 ? 1 : best);
 }
-int64_t rows_bytes(const Split &s, int groups, int h, int32_t max_pages) {
-  return s.rows ? static_cast<int64_t>(groups) * h * max_pages * 2 * xtc::kRowsBytes : 0;
-}
-int64_t partial_bytes(const Split &s, int64_t rows, int hq) {
-  return (s.chunks * rows * hq * (kDim + 1) * 4 + 255) / 256 * 256;
-}
+int64_t max_chunks(int32_t max_pages, int chunk) { return (max_pages + chunk - 1) / chunk; }
 
 template <int BITS, typename T>
-int launch(const PrefixArgs &a, const Split &s, cudaStream_t st) {
-  cudaLaunchAttribute behind{};  // a kernel that waits for the one before it itself
-  behind.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  behind.val.programmaticStreamSerializationAllowed = 1;
-  if (s.chunks > 0) {
+int launch(const PrefixArgs &a, int64_t chunks, cudaStream_t st) {
+  if (chunks > 0) {
+    auto kern = xtc::prefix_tc_kernel<BITS, T>;
     const int smem = static_cast<int>(sizeof(xtc::Smem<BITS>)) + 1024;
-    auto kern = s.rows ? xtc::prefix_tc_kernel<BITS, T, true> : xtc::prefix_tc_kernel<BITS, T, false>;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
       return NSNKV_ERR_CUDA;
-    xtc::Args x{a.q, a.records, a.table, a.n_pages, a.row_offsets, a.row_index, a.o_ws, a.e_ws, a.rows, a.pages,
-                a.table_stride, a.rec_head, a.rec_page, a.hq, a.h, a.max_pages, a.chunk_pages, a.row_tiles,
-                a.status, {}};
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(s.chunks), a.h, a.groups * a.row_tiles);
-    cfg.blockDim = dim3(xtc::kThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    if (s.rows) {
-      T *rows = reinterpret_cast<T *>(reinterpret_cast<uint8_t *>(a.o_ws) + partial_bytes(s, a.rows, a.hq));
-      const cuuint64_t dims[2] = {kDim, static_cast<cuuint64_t>(a.groups) * a.h * a.max_pages * 2 * kBlock};
-      const cuuint64_t strides[1] = {kDim * 2};
-      const cuuint32_t box[2] = {64, kBlock}, step[2] = {1, 1};
-      if (!tc::encoder() ||
-          tc::encoder()(&x.rows_map, Elem<T>::kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
-                        rows, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-        return NSNKV_ERR_CUDA;
-      xtc::prefix_restore_kernel<BITS, T><<<dim3(a.max_pages, a.h, a.groups), 128, 0, st>>>(x, rows);
-      if (cudaGetLastError() != cudaSuccess) return NSNKV_ERR_LAUNCH;
-      cfg.attrs = &behind;
-      cfg.numAttrs = 1;
-    }
-    if (cudaLaunchKernelEx(&cfg, kern, x) != cudaSuccess) return NSNKV_ERR_LAUNCH;
+    const xtc::Args x{a.q, a.records, a.table, a.n_pages, a.row_offsets, a.row_index, a.o_ws, a.e_ws, a.rows, a.pages,
+                      a.table_stride, a.rec_head, a.rec_page, a.hq, a.h, a.max_pages, a.chunk_pages, a.row_tiles,
+                      a.status};
+    kern<<<dim3(static_cast<unsigned>(chunks), a.h, a.groups * a.row_tiles), xtc::kThreads, smem, st>>>(x);
+    if (cudaGetLastError() != cudaSuccess) return NSNKV_ERR_LAUNCH;
   }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>((a.rows * a.hq + 3) / 4));
   cfg.blockDim = dim3(128);
   cfg.stream = st;
-  cfg.attrs = &behind;
-  cfg.numAttrs = s.chunks > 0 ? 1 : 0;  // only behind the chunk kernel, which announces it
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = chunks > 0 ? 1 : 0;  // only behind the chunk kernel, which announces it
   return cudaLaunchKernelEx(&cfg, prefix_merge_kernel<T>, a) == cudaSuccess ? NSNKV_OK : NSNKV_ERR_LAUNCH;
 }
 
@@ -196,8 +157,8 @@ extern "C" {
 
 int64_t nsnkv_prefix_attn_workspace_bytes(int64_t rows, int32_t groups, int hq, int h, int32_t max_pages) {
   if (rows <= 0 || groups <= 0 || hq <= 0 || h <= 0 || hq % h || max_pages < 0) return 0;
-  const Split s = split_for(rows, groups, hq / h, h, max_pages);
-  return partial_bytes(s, rows, hq) + rows_bytes(s, groups, h, max_pages);
+  const int64_t chunks = max_pages ? max_chunks(max_pages, chunk_pages_for(rows, groups, hq / h, h, max_pages)) : 0;
+  return chunks * rows * hq * (kDim + 1) * 4;
 }
 
 int nsnkv_prefix_attn(int64_t rows, int32_t groups, int64_t max_rows, int hq, int h, int bits, int dtype, const void *q,
@@ -222,18 +183,19 @@ int nsnkv_prefix_attn(int64_t rows, int32_t groups, int64_t max_rows, int hq, in
     return NSNKV_ERR_ARG;
   if (rows * hq > INT32_MAX || groups > 4096) return NSNKV_ERR_TOO_LARGE;
   const int G = hq / h;
-  const Split s = split_for(rows, groups, G, h, max_pages);
+  const int chunk = max_pages ? chunk_pages_for(rows, groups, G, h, max_pages) : 1;
+  const int64_t chunks = max_pages ? max_chunks(max_pages, chunk) : 0;
   if (max_rows <= 0 || max_rows > rows) max_rows = rows;
   int64_t tiles = (max_rows * G + kPairRows - 1) / kPairRows;
   if (tiles * groups > 65535) tiles = 65535 / groups;
   PrefixArgs a{q, records, table, n_pages, row_offsets, row_index, o_part, lse_part, out, lse,
-               static_cast<float *>(workspace), static_cast<float *>(workspace) + s.chunks * rows * hq * kDim,
-               rows, pages, table_stride, rec_stride_head, rec_stride_page, groups, hq, h, max_pages, s.chunk_pages,
+               static_cast<float *>(workspace), static_cast<float *>(workspace) + chunks * rows * hq * kDim,
+               rows, pages, table_stride, rec_stride_head, rec_stride_page, groups, hq, h, max_pages, chunk,
                static_cast<int32_t>(tiles), status};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (bits == 3)
-    return dtype == NSNKV_F16 ? launch<3, __half>(a, s, st) : launch<3, __nv_bfloat16>(a, s, st);
-  return dtype == NSNKV_F16 ? launch<5, __half>(a, s, st) : launch<5, __nv_bfloat16>(a, s, st);
+    return dtype == NSNKV_F16 ? launch<3, __half>(a, chunks, st) : launch<3, __nv_bfloat16>(a, chunks, st);
+  return dtype == NSNKV_F16 ? launch<5, __half>(a, chunks, st) : launch<5, __nv_bfloat16>(a, chunks, st);
 }
 
 }  // extern "C"

@@ -121,94 +121,9 @@ struct Args {
   int64_t rows, pages, table_stride, rec_head, rec_page;
   int32_t hq, h, max_pages, chunk_pages, pairs;
   int32_t *status;
-  // blocks restored ahead (prefix_restore_kernel): K rows of block i of group g, kv head j from row
-  // ((g * h + j) * 2 * max_pages + i) * 64 of a [..][128] array, its V rows max_pages blocks further
-  CUtensorMap rows_map;
 };
 
-// One block per CTA of 128 threads: the records of every group's prefix as rows of T.
 template <int BITS, typename T>
-__global__ void __launch_bounds__(128) prefix_restore_kernel(const __grid_constant__ Args a, T *rows) {
-  using R = rr::Rec<BITS>;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  __shared__ __align__(16) uint8_t rec[R::kBytes];
-  __shared__ __align__(16) float ab_s[2][2 * kDim];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, i = blockIdx.x, head = blockIdx.y, group = blockIdx.z;
-  const int np = min(max(a.n_pages ? a.n_pages[group] : a.max_pages, 0), a.max_pages);
-  if (i >= np) return;
-  int64_t page = a.table[group * a.table_stride + i];
-  if (page < 0 || page >= a.pages) {
-    if (tid == 0) set_status(a.status, NSNKV_ST_PAGE);
-    page = 0;
-  }
-  const uint4 *src4 = reinterpret_cast<const uint4 *>(a.records + head * a.rec_head + page * a.rec_page);
-#pragma unroll
-  for (int e = 0; e < (R::kBytes / 16 + 127) / 128; ++e)
-    if (tid + 128 * e < R::kBytes / 16) reinterpret_cast<uint4 *>(rec)[tid + 128 * e] = __ldcs(src4 + tid + 128 * e);
-  __syncthreads();
-  int bad = 0;
-  const float mul = __int_as_float((127 + 23 - Window<BITS>::bit(tid & 15)) << 23);
-#pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    const uint16_t *half = reinterpret_cast<const uint16_t *>(rec + x * R::kHalf + R::kMin) + tid;
-    const float p = half_bits_to_f(half[128]) * mul, y = half_bits_to_f(half[0]) - p;
-    bad |= !isfinite(y);
-    float *dst = &ab_s[x][2 * (tid & ~1)] + (tid & 1);
-    dst[0] = p;
-    dst[2] = y;
-  }
-  __syncthreads();
-  uint32_t one;
-  asm volatile("mov.u32 %0, 0x3F800000;" : "=r"(one));
-  const int g16 = lane & 7, r4 = warp * 4 + (lane >> 3);  // eight threads write a row's 256 bytes
-  const uint32_t sel = g16 & 1 ? 0x7632u : 0x5410u;
-  T *k_rows = rows + ((static_cast<int64_t>(group) * a.h + head) * 2 * a.max_pages + i) * kBlock * kDim + 16 * g16;
-  T *v_rows = k_rows + static_cast<int64_t>(a.max_pages) * kBlock * kDim;
-  float4 ab[8];
-  uint4 out[2];
-  uint32_t st[(BITS + 1) / 2], wd[BITS];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) ab[e] = reinterpret_cast<const float4 *>(ab_s[0])[8 * g16 + e];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const int t = r4 + 16 * e;
-    const uint32_t *src = reinterpret_cast<const uint32_t *>(rec) + t * 4 * BITS + (g16 >> 1) * BITS;
-    const float alpha = reinterpret_cast<const float *>(rec + R::kAlpha)[t];
-    bad |= !isfinite(alpha);
-#pragma unroll
-    for (int x = 0; x < BITS; ++x) wd[x] = src[x];
-#pragma unroll
-    for (int x = 0; x < (BITS + 1) / 2; ++x)
-      st[x] = __byte_perm(wd[2 * x], 2 * x + 1 < BITS ? wd[2 * x + 1] : 0u, sel);
-    values16<BITS, T>(st, ab, alpha, one, out);
-    reinterpret_cast<uint4 *>(k_rows + t * kDim)[0] = out[0];
-    reinterpret_cast<uint4 *>(k_rows + t * kDim)[1] = out[1];
-  }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) ab[e] = reinterpret_cast<const float4 *>(ab_s[1])[8 * g16 + e];
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int j = r4 + 16 * e;
-    const uint32_t *src = reinterpret_cast<const uint32_t *>(rec + R::kHalf) + j * 8 * BITS + g16 * BITS;
-    const float2 alpha = reinterpret_cast<const float2 *>(rec + R::kHalf + R::kAlpha)[j];
-    bad |= !isfinite(alpha.x) || !isfinite(alpha.y);
-#pragma unroll
-    for (int x = 0; x < BITS; ++x) wd[x] = src[x];
-#pragma unroll
-    for (int y = 0; y < 2; ++y) {
-#pragma unroll
-      for (int x = 0; x < (BITS + 1) / 2; ++x)
-        st[x] = __byte_perm(wd[2 * x], 2 * x + 1 < BITS ? wd[2 * x + 1] : 0u, y ? 0x7632u : 0x5410u);
-      values16<BITS, T>(st, ab, y ? alpha.y : alpha.x, one, out);
-      reinterpret_cast<uint4 *>(v_rows + (2 * j + y) * kDim)[0] = out[0];
-      reinterpret_cast<uint4 *>(v_rows + (2 * j + y) * kDim)[1] = out[1];
-    }
-  }
-  if (bad) set_status(a.status, NSNKV_ST_INPUT_NONFINITE);
-}
-
-// ROWS: the blocks were restored ahead and come by TMA; otherwise the CTA restores them.
-template <int BITS, typename T, bool ROWS>
 __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_constant__ Args a) {
   extern __shared__ uint8_t smem_raw[];
   using R = rr::Rec<BITS>;
@@ -226,7 +141,6 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
   }
   const int nrows = static_cast<int>(end - begin) * G;  // rows * hq fits an int
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge may take its place behind this grid
-  if constexpr (ROWS) asm volatile("griddepcontrol.wait;" ::: "memory");  // behind the restore kernel
   if (nloc <= 0 || (blockIdx.z % a.pairs) * 2 * kM >= nrows) return;
 
   if (warp == 16) {
@@ -453,7 +367,6 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
         }
       }
     } else if (warp < 16) {  // ---- restore
-      if constexpr (!ROWS) {
       // Two teams of four warps take alternate blocks, so that one works while the other waits
       // for its record, its tables or a free stage.
       const int team = (warp - 8) >> 2, w4 = warp & 3;
@@ -538,7 +451,6 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
         if (stage >= kStages) stage -= kStages, par ^= 1;
       }
       if (bad) set_status(a.status, NSNKV_ST_INPUT_NONFINITE);
-      }
     } else if (warp == 16) {  // ---- MMA: every lane runs the loops, one issues
       const bool lead = tc::elect();
       constexpr uint32_t kIdS = tc::instr_desc<T>(kM, kBlock, false), kIdO = tc::instr_desc<T>(kM, kDim, true);
@@ -603,26 +515,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
         }
       }
       __syncwarp();
-    } else if (ROWS && warp == 17) {  // ---- restored rows
-      const bool lead = tc::elect();
-      asm volatile("fence.proxy.async;" ::: "memory");  // the rows were written by ordinary stores
-      const int first_row = ((group * a.h + head) * 2 * a.max_pages + p0) * kBlock;
-#pragma unroll 1
-      for (int j = 0; j < nloc; ++j) {
-        const uint32_t n = blocks + j, stage = n % kStages;
-        tc::spin(&S.empty[stage], (n / kStages & 1) ^ 1, &S.failed, a.status);
-        if (lead) {
-          mbar_expect_tx(&S.full[stage], 2 * kRowsBytes);
-#pragma unroll
-          for (int x = 0; x < 4; ++x)  // K, V; channels 0 .. 63, 64 .. 127
-            tc::tma_load_2d(S.kv[stage][x >> 1] + (x & 1) * (kRowsBytes / 2), &a.rows_map, (x & 1) * 64,
-                            first_row + ((x >> 1) * a.max_pages + j) * kBlock, &S.full[stage]);
-        }
-      }
-      __syncwarp();
-      if (*static_cast<volatile int32_t *>(&S.failed))  // a wait gave up: let the copies in flight land
-        for (int i = 0; i < 1000; ++i) __nanosleep(1000);
-    } else if (!ROWS && warp == 17) {  // ---- records
+    } else if (warp == 17) {  // ---- records
       const int32_t *row = a.table + group * a.table_stride + p0;
       const bool lead = tc::elect();
       int32_t ids = 0;

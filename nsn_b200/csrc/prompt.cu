@@ -149,7 +149,14 @@ int launch_rows(const PromptArgs &a, int64_t longest, cudaStream_t st) {
 // Tensor map of x [tokens][heads][128] with element strides: boxes of 64 channels of one
 // head and 128 tokens, 128-byte swizzle.
 bool make_map(CUtensorMap *map, const void *base, int dtype, int64_t tokens, int heads, int64_t tok, int64_t head) {
-  const auto encode = tc::encoder();
+  static const auto encode = [] {
+    void *fn = nullptr;
+    cudaDriverEntryPointQueryResult got;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &got) != cudaSuccess ||
+        got != cudaDriverEntryPointSuccess)
+      fn = nullptr;
+    return reinterpret_cast<decltype(&cuTensorMapEncodeTiled)>(fn);
+  }();
   if (!encode) return false;
   const cuuint64_t dims[3] = {kDim, static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(tokens)};
   // the stride of a dimension of one element is never used
