@@ -109,7 +109,7 @@ def case(h, G, bits, dtype, counts, per_group, seed=0, part=True, spare=2, loose
 @pytest.mark.parametrize("h,G,counts,per_group", [
     (2, 4, [1], [1]), (1, 1, [3], [1]), (2, 2, [5], [70]), (3, 3, [2], [17]), (2, 8, [9], [9]), (1, 4, [33], [40]),
     (2, 4, [4, 1, 7], [3, 9, 1]), (2, 4, [0, 3], [4, 4]), (1, 6, [2, 2], [1, 60]), (8, 4, [20], [2]),
-    (2, 1, [130], [2]), (1, 16, [6], [20])])
+    (2, 1, [130], [2]), (1, 16, [6], [20]), (1, 4, [5], [300]), (1, 8, [3, 6], [150, 200]), (2, 6, [7, 0], [260, 9])])
 def test_groups_and_lengths(h, G, counts, per_group, bits, dtype):
     from nsn_b200.prefix import prefix_attention
     a, kw, ref = case(h, G, bits, dtype, counts, per_group)

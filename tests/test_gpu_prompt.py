@@ -64,7 +64,8 @@ def check(out, lse, ref, rows=slice(None)):
 
 
 LENS = [[1], [2], [63], [64], [65], [127], [128], [129], [255], [256], [257], [3, 0, 130, 1, 64, 511], [1] * 37,
-        [1500], [700, 1, 900]]
+        [1500], [700, 1, 900],
+        [66] * 140]  # more sequences than the longest-first order keeps in registers
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
