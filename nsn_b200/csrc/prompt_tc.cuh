@@ -14,6 +14,13 @@
 // tensor core adds P.V to O, P read from TMEM.  While one row tile is in its softmax the
 // tensor core works on the other.
 //
+// Measured: 16384 tokens, GQA 32:8, fp16: 1.79 ms in a short run (1230 TFLOP/s, 0.75 of the
+// library GEMM's burst rate), 2.15 ms under sustained load, where the power limit holds the clock;
+// 4 x 2048 tokens, 16 heads: 100 us.  What bounds it is the chain S -> softmax -> P.V of one row
+// tile with one warp per scheduler (about 2450 of 3150 cycles per K / V tile are softmax); the
+// tensor pipe is busy 43% to 50% of the time.  Tiles are 128 tokens because Q.K^T with both operands in shared
+// memory reads 128 bytes a cycle at N = 128, all that shared memory gives, and more below.
+//
 // The running maximum m is only raised when a row's maximum passed it by more than 8 (in log2
 // units): p stays below 2^8, l and O are then in units of the stale maximum, which cancels in
 // O / l, and O (in TMEM) is rescaled rarely instead of once per tile.

@@ -107,6 +107,20 @@ def test_head_major_strides():
     check(out, lse, reference(q, k, v, lens))
 
 
+@pytest.mark.parametrize("lens", [[40], [300, 45]], ids=str)
+def test_broadcast_heads_and_unaligned_output(lens):
+    """K and V of one head expanded to four (stride 0), and an output that is only 16-byte aligned."""
+    from nsn_b200.prompt import prompt_attention
+    q, k, v, cu = make(lens, 4, 1, torch.float16)
+    ref = reference(q, k, v, lens)
+    T = sum(lens)
+    wide = prompt_attention(q, k.expand(T, 4, 128), v.expand(T, 4, 128), cu, max(lens))
+    check(*wide, ref)
+    out = torch.empty(T * 512 + 8, dtype=torch.float16, device="cuda")[8:].view(T, 4, 128)
+    prompt_attention(q, k, v, cu, max(lens), out=out)
+    check(out, wide[1], ref)
+
+
 @pytest.mark.parametrize("longest", [1, 64, 100000])
 def test_longest_only_sizes_the_launch(longest):
     from nsn_b200.prompt import prompt_attention
