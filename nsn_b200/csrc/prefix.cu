@@ -128,8 +128,8 @@ int launch(const PrefixArgs &a, int64_t chunks, cudaStream_t st) {
   if (chunks > 0) {
     auto kern = xtc::prefix_tc_kernel<BITS, T>;
     const int smem = static_cast<int>(sizeof(xtc::Smem<BITS>)) + 1024;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-      return NSNKV_ERR_CUDA;
+    static std::atomic<uint64_t> done{0};
+    if (!allow_smem(kern, smem, done)) return NSNKV_ERR_CUDA;
     const xtc::Args x{a.q, a.records, a.table, a.n_pages, a.row_offsets, a.row_index, a.o_ws, a.e_ws, a.rows, a.pages,
                       a.table_stride, a.rec_head, a.rec_page, a.hq, a.h, a.max_pages, a.chunk_pages, a.row_tiles,
                       a.status};

@@ -140,8 +140,8 @@ __global__ void __launch_bounds__(128, 3) prompt_rows_kernel(const PromptArgs a)
 template <typename T>
 int launch_rows(const PromptArgs &a, int64_t longest, cudaStream_t st) {
   auto kern = prompt_rows_kernel<T>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(RowsSmem)) != cudaSuccess)
-    return NSNKV_ERR_CUDA;
+  static std::atomic<uint64_t> done{0};
+  if (!allow_smem(kern, sizeof(RowsSmem), done)) return NSNKV_ERR_CUDA;
   const int64_t tiles = (longest + kRowsCta - 1) / kRowsCta;
   const dim3 grid(static_cast<unsigned>(tiles < 65535 ? tiles : 65535), a.hq, a.seqs);
   kern<<<grid, 128, sizeof(RowsSmem), st>>>(a);
@@ -182,8 +182,8 @@ int launch_tc(const PromptArgs &p, int dtype, cudaStream_t st) {
                     p.v_head, p.seqs, p.hq, p.h, p.causal, p.status};
   auto kern = ptc::prompt_tc_kernel<T>;
   const int smem = static_cast<int>(sizeof(ptc::Smem)) + 1024;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return NSNKV_ERR_CUDA;
+  static std::atomic<uint64_t> done{0};
+  if (!allow_smem(kern, smem, done)) return NSNKV_ERR_CUDA;
   // at most one pair of row tiles per 256 tokens and one more per sequence
   const int64_t items = (p.tokens / (2 * ptc::kM) + p.seqs) * p.hq;
   kern<<<static_cast<unsigned>(items < kSms ? items : kSms), ptc::kThreads, smem, st>>>(a, maps);

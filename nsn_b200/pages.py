@@ -134,10 +134,10 @@ def compact_pages(arrays, block_table, page_refs, table_out=None, refs_out=None,
     """
     dev, (batch, max_blocks) = block_table.device, block_table.shape
     if table_out is None:
-        table_out = torch.empty((batch, max_blocks), dtype=torch.int32, device=dev)
+        table_out = block_table.new_empty((batch, max_blocks))
     if refs_out is None:
         refs_out = torch.empty_like(page_refs)
-    live = torch.empty(1, dtype=torch.int32, device=dev)
+    live = page_refs.new_empty(1)
     _ints("compact_pages", dev, block_table, page_refs, table_out, refs_out)
     h, pages, arr = _page_arrays(arrays, dev)
     if not (page_refs.shape == refs_out.shape == (pages,) and table_out.shape == block_table.shape):

@@ -66,11 +66,11 @@ def prefix_attention(q, records, page_table, n_pages=None, *, bits=3, row_offset
             raise w.ContractError("prefix attention partial: fp32 o_part [rows, hq, 128] with lse_part [rows, hq]")
         o_ptr, e_ptr = o_part.data_ptr(), lse_part.data_ptr()
     if out is None:
-        out = torch.empty(qs, dtype=dt, device=dev)
+        out = torch.empty_like(q)
     elif not (out.shape == qs and out.dtype == dt and out.is_contiguous() and out.device == dev):
         raise w.ContractError("prefix attention out: contiguous, of q's shape, dtype and device")
     if lse is None:
-        lse = torch.empty((rows, hq), dtype=torch.float32, device=dev)
+        lse = q.new_empty((rows, hq), dtype=torch.float32) if lse_part is None else torch.empty_like(lse_part)
     elif not (lse.shape == qs[:2] and lse.dtype == torch.float32 and lse.is_contiguous() and lse.device == dev):
         raise w.ContractError("prefix attention lse: contiguous fp32 [rows, hq] on q's device")
     lib, index = L.load(), dev.index

@@ -41,11 +41,11 @@ def prompt_attention(q, k, v, cu_seqlens, max_seqlen, *, causal=True, out=None, 
     if not (qc == kc == vc == 1 and not (qt | qh | kt | kh | vt | vh) & 7 and not (qp | kp | vp) & 15):
         raise w.ContractError("prompt attention strides: contiguous channels, strides multiples of 8, 16-byte aligned")
     if out is None:
-        out = torch.empty(qs, dtype=dt, device=dev)
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(qs)
     elif not (out.shape == qs and out.dtype == dt and out.is_contiguous() and out.device == dev):
         raise w.ContractError("prompt attention out: contiguous, of q's shape, dtype and device")
     if lse is None:
-        lse = torch.empty((T, hq), dtype=torch.float32, device=dev)
+        lse = q.new_empty((T, hq), dtype=torch.float32)
     elif not (lse.shape == (T, hq) and lse.dtype == torch.float32 and lse.is_contiguous() and lse.device == dev):
         raise w.ContractError("prompt attention lse: contiguous fp32 [T, hq] on q's device")
     index = dev.index
