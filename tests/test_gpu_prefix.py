@@ -184,7 +184,8 @@ def test_statuses():
         if what == "page":
             t[0, 1] = rec.shape[1]
         if what == "meta":
-            rec[0, int(t[0, 2]), 3072:3074] = 255  # a channel's min: NaN
+            at = rec.shape[2] // 2 - 768  # behind K's codes: the channels' minima
+            rec[0, int(t[0, 2]), at:at + 2] = 255  # NaN
         if what == "q":
             q[1, 0, 5] = math.inf
         prefix_attention(q, rec, t, n, status=status, **kw)
