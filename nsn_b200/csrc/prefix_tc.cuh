@@ -18,9 +18,9 @@
 // not below 2^-24 of a (true of unit directions: min and scale within a few powers of two);
 // elsewhere it is within 2^-24 a of it.  a and b are laid out once per block and channel.
 //
-// Measured: 64 rows over 8192 INT3 tokens, GQA 32:8: 34.8 us with the merge (eight blocks per CTA at
+// Measured: 64 rows over 8192 INT3 tokens, GQA 32:8: 35.4 us with the merge (eight blocks per CTA at
 // 2400 cycles between a start of 9 k cycles and 8 k of writing partial rows); 8 rows over 131008
-// INT5 tokens, GQA 64:8: 152 us (1.26 TB/s of records, 0.5 instructions per cycle and scheduler).
+// INT5 tokens, GQA 64:8: 156 us (1.24 TB/s of records, 0.5 instructions per cycle and scheduler).
 // Blocks of 64 tokens, not 128, leave TMEM for two buffers of S per team and shared memory for
 // four restored blocks.
 #pragma once
@@ -34,9 +34,6 @@ namespace xtc {
 
 constexpr int kM = 128;
 constexpr int kThreads = 640;
-// A maximum is taken this much (log2 units) above the block's: scores may grow by 2^21 before
-// the next raise, and p of the largest, 2^-6, leaves fp16's 2^-24 far below its rounding.
-constexpr float kHeadroom = 6.f;
 constexpr int kStages = 4;  // restored blocks held
 constexpr int kStageRow = kDim * 4 + 16;  // a staged output row (bytes)
 constexpr int kRowsBytes = kBlock * kDim * 2;  // K or V of one block
@@ -267,7 +264,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
           for (int again = j == 0;; again = 1) {
             fetch();
             if (again) {
-              const float m_new = fmaxf(m, top() + kHeadroom);
+              const float m_new = fmaxf(m, top());
               const float c = m_new == -INFINITY ? 1.f : fm::ex2(m - m_new);
               if (j > 0) {
                 tc::spin(&S.o_done[t], (n - 1) & 1, &S.failed, a.status);  // P.V of the block before

@@ -126,6 +126,17 @@ def test_row_tiles(rows):
     check(prefix_attention(*a, **kw), ref)
 
 
+@pytest.mark.parametrize("bits,counts,rows", [(3, [3], [300]), (5, [4, 5], [70, 200]), (3, [1], [97])])
+def test_max_rows_only_sizes_the_launch(bits, counts, rows):
+    """Fewer row tiles launched than the groups have: a CTA takes several in turn."""
+    from nsn_b200.prefix import prefix_attention
+    a, kw, ref = case(1, 4, bits, torch.float16, counts, rows, seed=9)
+    kw["max_rows"] = 1
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    check(prefix_attention(*a, status=status, **kw), ref)
+    assert int(status) == 0
+
+
 def test_rows_outside_every_group_and_no_partial():
     from nsn_b200.prefix import prefix_attention
     a, kw, ref = case(2, 4, 3, torch.float16, [3, 2], [2, 3], loose=4)
