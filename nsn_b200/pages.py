@@ -16,13 +16,16 @@ import torch
 from . import _lib as L
 from . import primitives as w
 
+_I32 = torch.int32
 _ARRAYS = {n: L.PageArray * n for n in range(1, 9)}
 
 
 def _ints(name, dev, *tensors):
+    ok = dev.type == "cuda"
     for t in tensors:
-        if not (t.dtype == torch.int32 and t.device == dev and t.is_cuda and (t.numel() <= 1 or t.stride(-1) == 1)):
-            raise w.ContractError(f"{name}: int32 CUDA tensors on one device")
+        ok = ok and t.dtype == _I32 and t.device == dev and (t.is_contiguous() or t.stride(-1) == 1)
+    if not ok:
+        raise w.ContractError(f"{name}: int32 CUDA tensors on one device")
 
 
 def _p(t):
@@ -92,17 +95,13 @@ def _page_arrays(arrays, dev):
     lead = arrays[0].shape[:2] if got is not None else None
     for i, t in enumerate(arrays):
         shape, stride, size = t.shape, t.stride(), t.element_size()
-        n = size
+        n = 1
         for d in range(len(shape) - 1, 1, -1):  # contiguous pages
-            if stride[d] * size != n and shape[d] != 1:
-                n = -1
-                break
-            n *= shape[d]
+            n = n * shape[d] if stride[d] == n or shape[d] == 1 else -1
         if got is None or len(shape) < 3 or shape[:2] != lead or t.device != dev or n <= 0:
             got = None
             break
-        a = got[i]
-        a.base, a.bytes, a.stride_head, a.stride_page = t.data_ptr(), n, stride[0] * size, stride[1] * size
+        got[i] = (t.data_ptr(), n * size, stride[0] * size, stride[1] * size)
     if got is None:
         raise w.ContractError("page arrays: one to eight [h, pages, ...] tensors of one device with contiguous pages")
     return lead[0], lead[1], got
