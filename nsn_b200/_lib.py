@@ -179,14 +179,26 @@ def raw_stream(index: int) -> int:
 _scratch: dict = {}
 
 
+def capturing(index: int) -> bool:
+    """Whether the current stream of device `index` is being captured into a graph."""
+    if torch.cuda.current_device() == index:
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(index):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def scratch(nbytes: int, device, stream: int) -> torch.Tensor:
     """Reusable device scratch of at least `nbytes`, one buffer per (device, stream): calls on one
-    stream run in order and may share it, calls on different streams get different ones."""
+    stream run in order and may share it, calls on different streams get different ones.
+
+    A captured call gets a buffer of its own from the graph's memory, never a shared one: the
+    graph keeps the address, while a shared buffer is freed when a larger call replaces it and
+    is written by eager calls while the graph replays on another stream."""
+    if capturing(device.index):
+        return torch.empty(max(nbytes, 1), dtype=torch.uint8, device=device)
     buf = _scratch.get((device.index, stream))
     if buf is None or buf.numel() < nbytes:
-        buf = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
-        if not torch.cuda.is_current_stream_capturing():  # a captured call's buffer belongs to its graph
-            _scratch[(device.index, stream)] = buf
+        buf = _scratch[(device.index, stream)] = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
     return buf
 
 

@@ -239,3 +239,36 @@ def test_refusals():
             prefix_attention(a["q"], a["rec"], a["t"], a["n"], **b)
     with pytest.raises(NativeError):
         prefix_attention(q, rec, t, n, ws=torch.empty(16, dtype=torch.uint8, device="cuda"), **kw)
+
+
+def test_a_graph_keeps_its_workspace():
+    """Warmed up and captured on one stream, a larger eager call there afterwards, and new tensors
+    where its old buffer was: a replay gives what the call gave and writes nothing else."""
+    from nsn_b200.prefix import prefix_attention
+    a, kw, ref = case(2, 4, 3, torch.float16, [40], [33])
+    b, kb, big = case(2, 4, 3, torch.float16, [30], [300], seed=2)
+    out, lse = torch.empty_like(a[0]), torch.empty((33, 8), device="cuda")
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(s):
+        prefix_attention(*a, out=out, lse=lse, **kw)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=s):
+        prefix_attention(*a, out=out, lse=lse, **kw)
+    with torch.cuda.stream(s):
+        check(prefix_attention(*b, **kb), big)
+        others = [torch.full((1 << 18,), 7.0, device="cuda") for _ in range(64)]
+        out.zero_()
+        graph.replay()
+    s.synchronize()
+    check((out, lse), ref)
+    assert all(bool((x == 7).all()) for x in others)
+    with torch.cuda.stream(s):  # eager calls there while the graph replays elsewhere
+        got = [prefix_attention(*b, **kb) for _ in range(20)]
+    for _ in range(20):
+        graph.replay()
+    torch.cuda.synchronize()
+    check((out, lse), ref)
+    for x in got:
+        check(x, big)

@@ -1,0 +1,35 @@
+"""The operators' default device scratch: who may share a buffer and who may not."""
+import pytest
+import torch
+
+CPU = torch.device("cpu", 0)  # the bookkeeping is the same on any device
+
+
+@pytest.fixture
+def capturing(monkeypatch):
+    """A switch for "the current stream is being captured"; device 0 is current."""
+    state = {"on": False}
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: state["on"])
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    return state
+
+
+def test_calls_on_one_stream_share_a_buffer(capturing):
+    from nsn_b200 import _lib as L
+    a = L.scratch(1 << 10, CPU, 901)
+    assert L.scratch(1 << 12, CPU, 901).data_ptr() == a.data_ptr()
+    assert L.scratch(1 << 12, CPU, 902).data_ptr() != a.data_ptr()
+    b = L.scratch(1 << 21, CPU, 901)
+    assert b.numel() >= 1 << 21 and L.scratch(16, CPU, 901).data_ptr() == b.data_ptr()
+
+
+def test_a_captured_call_never_gets_an_eager_buffer(capturing):
+    """A graph keeps the addresses it was captured with, so its buffer must be its own: an eager
+    buffer is replaced (and freed) when it grows, and is written by eager calls during a replay."""
+    from nsn_b200 import _lib as L
+    eager = L.scratch(1 << 10, CPU, 903)
+    capturing["on"] = True
+    graph = L.scratch(1 << 10, CPU, 903)
+    assert graph.data_ptr() != eager.data_ptr()
+    capturing["on"] = False
+    assert L.scratch(1 << 10, CPU, 903).data_ptr() == eager.data_ptr()
