@@ -7,6 +7,7 @@ current torch CUDA stream.
 from __future__ import annotations
 
 import ctypes
+import threading
 from ctypes import c_int, c_int32, c_int64, c_void_p
 from pathlib import Path
 
@@ -176,7 +177,12 @@ def raw_stream(index: int) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
-_scratch: dict = {}
+class _Scratch(threading.local):
+    def __init__(self):
+        self.held = {}
+
+
+_scratch = _Scratch()
 
 
 def capturing(index: int) -> bool:
@@ -188,17 +194,20 @@ def capturing(index: int) -> bool:
 
 
 def scratch(nbytes: int, device, stream: int) -> torch.Tensor:
-    """Reusable device scratch of at least `nbytes`, one buffer per (device, stream): calls on one
-    stream run in order and may share it, calls on different streams get different ones.
+    """Reusable device scratch of at least `nbytes`, one buffer per host thread, device and stream:
+    one thread's calls on a stream run in order and may share it.  Calls on different streams get
+    different ones, and so do threads on one stream, since an operator's second kernel may be
+    enqueued behind another thread's first.
 
     A captured call gets a buffer of its own from the graph's memory, never a shared one: the
     graph keeps the address, while a shared buffer is freed when a larger call replaces it and
     is written by eager calls while the graph replays on another stream."""
     if capturing(device.index):
         return torch.empty(max(nbytes, 1), dtype=torch.uint8, device=device)
-    buf = _scratch.get((device.index, stream))
+    held = _scratch.held
+    buf = held.get((device.index, stream))
     if buf is None or buf.numel() < nbytes:
-        buf = _scratch[(device.index, stream)] = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
+        buf = held[(device.index, stream)] = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
     return buf
 
 

@@ -272,3 +272,25 @@ def test_a_graph_keeps_its_workspace():
     check((out, lse), ref)
     for x in got:
         check(x, big)
+
+
+def test_threads_on_one_stream():
+    """Two host threads enqueue on the same stream; each call joins its own chunks."""
+    import threading
+    from nsn_b200.prefix import prefix_attention
+    cases = [case(2, 4, 3, torch.float16, [40], [33], seed=s) for s in (1, 2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def run(i):
+        a, kw, _ = cases[i]
+        got[i] += [prefix_attention(*a, **kw) for _ in range(200)]
+    threads = [threading.Thread(target=run, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        check(got[i][0], cases[i][2])
+        assert all(torch.equal(o, got[i][0][0]) and torch.equal(e, got[i][0][1]) for o, e in got[i])

@@ -1,4 +1,6 @@
 """The operators' default device scratch: who may share a buffer and who may not."""
+import threading
+
 import pytest
 import torch
 
@@ -33,3 +35,13 @@ def test_a_captured_call_never_gets_an_eager_buffer(capturing):
     assert graph.data_ptr() != eager.data_ptr()
     capturing["on"] = False
     assert L.scratch(1 << 10, CPU, 903).data_ptr() == eager.data_ptr()
+
+
+def test_host_threads_on_one_stream_do_not_share(capturing):
+    """An operator enqueues two kernels; another thread's may come between them."""
+    from nsn_b200 import _lib as L
+    mine, other = L.scratch(1 << 10, CPU, 904), []
+    t = threading.Thread(target=lambda: other.append(L.scratch(1 << 10, CPU, 904)))
+    t.start()
+    t.join()
+    assert other[0].data_ptr() != mine.data_ptr()
