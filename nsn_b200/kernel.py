@@ -30,25 +30,13 @@ attention_launch_count = 0
 FUSED_ARMS = ("V_FUSED", "GQA_FUSED")
 TILE_ARMS = ("TILE_MATERIALIZE", "TILE_SDPA", "RF01_MATERIALIZE")
 
-_workspace_cache: dict = {}
-
 
 def workspace(nbytes: int, device) -> torch.Tensor:
-    """Reusable scratch for the split-KV partials, one buffer per (device, current stream).
-
-    Calls on one stream run in order, so they can share a buffer; calls on different
-    streams get different buffers and never race on the partials.  A buffer that grows is
-    replaced on its own stream only, where every earlier call has been ordered before the
-    caching allocator can hand the old memory out again.
-    """
+    """Reusable scratch for the split-KV partials on the current stream (_lib.scratch)."""
     device = torch.device(device)
-    stream = torch.cuda.current_stream(device)
-    key = (str(device), stream.cuda_stream)
-    buf = _workspace_cache.get(key)
-    if buf is None or buf.numel() < nbytes:
-        buf = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
-        _workspace_cache[key] = buf
-    return buf
+    if device.type == "cuda" and device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
+    return L.scratch(nbytes, device, torch.cuda.current_stream(device).cuda_stream)
 
 
 def decode_attention(q, k_pool, v_pool, *, h, bits, blk_stride_head, blk_stride_page, n_blocks, max_blocks,

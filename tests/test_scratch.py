@@ -45,3 +45,14 @@ def test_host_threads_on_one_stream_do_not_share(capturing):
     t.start()
     t.join()
     assert other[0].data_ptr() != mine.data_ptr()
+
+
+def test_decode_attention_in_a_graph(capturing, monkeypatch):
+    """The decode kernels' default workspace keeps the same rules."""
+    from types import SimpleNamespace
+    from nsn_b200 import kernel
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: SimpleNamespace(cuda_stream=905))
+    eager = kernel.workspace(1 << 10, CPU)
+    assert kernel.workspace(1 << 9, CPU).data_ptr() == eager.data_ptr()
+    capturing["on"] = True
+    assert kernel.workspace(1 << 10, CPU).data_ptr() != eager.data_ptr()
