@@ -219,17 +219,19 @@ struct Rows {
     }
   }
 
-  // Row sums over the four lanes of a row; inv: 1 / l (0 for a row that saw nothing).
+  // Row sums over the four lanes of a row; inv: 1 / l.  l is 0 for a row that saw nothing (any
+  // finite score leaves at least one p near 1) and NaN for one whose scores are all NaN, though m,
+  // a maximum that passes NaN over, is -inf in both.
   __device__ __forceinline__ void finish(float (&inv)[2]) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
       l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-      inv[i] = m[i] == -INFINITY ? 0.f : __fdiv_rn(1.f, l[i]);
+      inv[i] = l[i] == 0.f ? 0.f : __fdiv_rn(1.f, l[i]);
     }
   }
   // Log-sum-exp of row i of this lane (base 2), -inf for a row that saw nothing.
-  __device__ __forceinline__ float lse2(int i) const { return m[i] == -INFINITY ? -INFINITY : m[i] + log2f(l[i]); }
+  __device__ __forceinline__ float lse2(int i) const { return l[i] == 0.f ? -INFINITY : m[i] + log2f(l[i]); }
 };
 
 }  // namespace fm

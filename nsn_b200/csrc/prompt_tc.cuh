@@ -532,7 +532,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::wait(&S.o_full[t], taken & 1, &S.failed, a.status);
       ++taken;
       tc::fence_after();
-      const float inv = m == -INFINITY ? 0.f : __fdiv_rn(1.f, l);
+      const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);  // l: 0 if the row saw nothing, NaN if only NaN
       const uint32_t o_at = tmem + (static_cast<uint32_t>(warp & 3) << 21) + 256 + 128 * t;
       const int64_t at = static_cast<int64_t>(it.begin + row) * a.hq + it.head;
       T *orow = static_cast<T *>(a.out) + at * kDim;
@@ -558,7 +558,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::fence_before();  // O is read before the next item's first P is announced
       if (row < it.len) {
         if (check.x + check.y != 0.f) atomicOr(&S.redo[t][k >> 5 & 31], 1u << (k & 31));
-        if (a.lse) a.lse[at] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * fm::kLn2;
+        if (a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * fm::kLn2;
       }
     }
   }

@@ -228,3 +228,23 @@ def test_refusals():
     wide = torch.zeros((64, 4, 132), dtype=torch.float16, device="cuda")
     with pytest.raises(ContractError):
         prompt_attention(wide[..., 1:129], k, v, cu, 64)
+
+
+@pytest.mark.parametrize("lens", [[40, 13], [300, 45]], ids=str)
+@pytest.mark.parametrize("where", ["q", "k"])
+def test_a_row_without_a_finite_score_is_nan(lens, where):
+    """A row whose scores are all NaN has a NaN output and log-sum-exp, not those of a row that
+    sees nothing; the other rows keep theirs."""
+    from nsn_b200.prompt import prompt_attention
+    q, k, v, cu = make(lens, 4, 2, torch.float16)
+    ref = reference(q, k, v, lens)
+    bad = torch.zeros(sum(lens), dtype=torch.bool, device="cuda")
+    if where == "q":
+        q[20] = math.nan
+        bad[20] = True
+    else:  # the second sequence's first token: every row of it sees it, its first row nothing else
+        k[lens[0]] = math.nan
+        bad[lens[0]:] = True
+    out, lse = prompt_attention(q, k, v, cu, max(lens))
+    assert bool(out[bad].isnan().all()) and bool(lse[bad].isnan().all())
+    check(out, lse, ref, ~bad)
