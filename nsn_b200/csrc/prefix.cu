@@ -43,7 +43,9 @@ __device__ __forceinline__ int64_t row_at(const PrefixArgs &a, int64_t p) {
 }
 
 // One warp per (query row, head): the chunks of its group and its own partial.  Lane c holds
-// chunk c's log-sum-exp; the chunks' rows are read four at a time.
+// chunk c's log-sum-exp; the chunks' rows are read four at a time.  A part with log-sum-exp -inf
+// holds nothing and is left out; one with NaN makes the row NaN (the sum of weights l becomes NaN,
+// while the maximum passes NaN over).
 template <typename T>
 __global__ void __launch_bounds__(128) prefix_merge_kernel(const PrefixArgs a) {
   asm volatile("griddepcontrol.wait;" ::: "memory");  // launched while the chunk kernel runs
@@ -65,7 +67,7 @@ __global__ void __launch_bounds__(128) prefix_merge_kernel(const PrefixArgs a) {
   const float own = a.lse_part ? a.lse_part[at] * fm::kLog2e : -INFINITY;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   if (own != -INFINITY) o = reinterpret_cast<const float4 *>(a.o_part + at * kDim)[lane];  // else it is not read
-  float m = own, l = own == -INFINITY ? 0.f : 1.f;
+  float m = own, l = own == -INFINITY ? 0.f : isnan(own) ? own : 1.f;
   for (int c0 = 0; c0 < chunks; c0 += 32) {
     const float e = c0 + lane < chunks ? a.e_ws[(c0 + lane) * step + at] : -INFINITY;
     float top = e;
@@ -97,13 +99,13 @@ __global__ void __launch_bounds__(128) prefix_merge_kernel(const PrefixArgs a) {
       }
     }
   }
-  const float inv = m == -INFINITY ? 0.f : __fdiv_rn(1.f, l);
+  const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
   const uint2 w = make_uint2(fm::round_pair<T>(o.x * inv, o.y * inv), fm::round_pair<T>(o.z * inv, o.w * inv));
   reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + at * kDim)[lane] = w;
   const float2 x = Elem<T>::to_f2(w.x), y = Elem<T>::to_f2(w.y);
   if (!isfinite(x.x) || !isfinite(x.y) || !isfinite(y.x) || !isfinite(y.y))
     set_status(a.status, NSNKV_ST_OUTPUT_NONFINITE);
-  if (a.lse && lane == 0) a.lse[at] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * fm::kLn2;
+  if (a.lse && lane == 0) a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * fm::kLn2;
 }
 
 constexpr int kSms = 148;

@@ -311,7 +311,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
         if (r < nrows) qr = a.row_index ? a.row_index[begin + pr] : begin + pr;
         const bool mine = qr >= 0 && qr < a.rows;
         const int64_t at = (blockIdx.x * a.rows + qr) * a.hq + head * G + (r - pr * G);
-        float inv = m == -INFINITY ? 0.f : __fdiv_rn(1.f, l), e2 = m == -INFINITY ? -INFINITY : m + log2f(l);
+        // l is 0 where the team had no block and NaN where every score is NaN, though m, a maximum
+        // that passes NaN over, is -inf in both
+        float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l), e2 = l == 0.f ? -INFINITY : m + log2f(l);
         // Both teams have seen their last P.V: every MMA is done, and Q and the ring are free.  Team
         // 1's half of a shared tile goes to team 0 through them, column by column of all rows;
         // finished rows are staged there and leave in one bulk copy each (rows 16 bytes apart
@@ -324,10 +326,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
           tc::bar_named(4, 256);
           const float e1 = S.e_other[tid & 127], top = fmaxf(e2, e1), b0 = top == -INFINITY ? 0.f : top;
           const float x0 = e2 == -INFINITY ? 0.f : fm::ex2(e2 - b0), x1 = e1 == -INFINITY ? 0.f : fm::ex2(e1 - b0);
-          const float is = top == -INFINITY ? 0.f : __fdiv_rn(1.f, x0 + x1);
+          const float both = x0 + x1, is = both == 0.f ? 0.f : __fdiv_rn(1.f, both);
           inv *= x0 * is;
           w = x1 * is;
-          e2 = top == -INFINITY ? -INFINITY : top + log2f(x0 + x1);
+          e2 = both == 0.f ? -INFINITY : top + log2f(both);
         }
         if (!split || t == 0 || team_blocks[1]) {
 #pragma unroll 1

@@ -294,3 +294,31 @@ def test_threads_on_one_stream():
     for i in (0, 1):
         check(got[i][0], cases[i][2])
         assert all(torch.equal(o, got[i][0][0]) and torch.equal(e, got[i][0][1]) for o, e in got[i])
+
+
+@pytest.mark.parametrize("blocks,rows,part", [(1, 3, True), (1, 3, False), (40, 3, True), (2, 70, True), (0, 3, True)])
+def test_a_row_without_a_finite_score_is_nan(blocks, rows, part):
+    """A NaN query's output and log-sum-exp are NaN over any prefix, with its own finite part or
+    without; the other rows keep theirs."""
+    from nsn_b200.prefix import prefix_attention
+    a, kw, ref = case(1, 4, 3, torch.float16, [blocks], [rows], part=part)
+    a[0][1] = math.nan
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out, lse = prefix_attention(*a, status=status, **kw)
+    if blocks:
+        assert bool(out[1].isnan().all()) and bool(lse[1].isnan().all()) and int(status) & 1
+    keep = torch.arange(rows, device="cuda") != 1 if blocks else slice(None)  # no prefix: q is not read
+    check((out[keep], lse[keep]), [t[keep] for t in ref])
+
+
+@pytest.mark.parametrize("blocks", [0, 3])
+def test_a_nan_part_is_not_dropped(blocks):
+    """A row whose own part has a NaN log-sum-exp is NaN: NaN does not mean "no own tokens"."""
+    from nsn_b200.prefix import prefix_attention
+    a, kw, ref = case(1, 4, 3, torch.float16, [blocks], [5])
+    kw["o_part"][2], kw["lse_part"][2] = math.nan, math.nan
+    kw["lse_part"][3] = math.nan  # its output finite
+    out, lse = prefix_attention(*a, **kw)
+    assert bool(out[2:4].isnan().all()) and bool(lse[2:4].isnan().all())
+    keep = torch.tensor([0, 1, 4], device="cuda")
+    check((out[keep], lse[keep]), [t[keep] for t in ref])
