@@ -29,7 +29,10 @@ from .prompt import prompt_attention
 
 class SharedPrefix:
     """Which sequences of a cache share which leading pages, laid out for its step_shared
-    (made by SharedPagedKVCache.share; valid until a fork, free, prefill or compaction)."""
+    (made by SharedPagedKVCache.share; valid until a fork, free, prefill, import or compaction).
+
+    ``own_table`` is a copy of the block table's entries behind the prefixes; step_shared brings it
+    up to date when pages were assigned since (by any step, a seal, extend or reserve)."""
 
     def __init__(self, cache, groups):
         batch, dev = cache.batch, cache.device
@@ -68,6 +71,7 @@ class SharedPrefix:
 
     def refresh(self, cache):
         torch.gather(cache.block_table, 1, self.own_at, out=self.own_table)
+        self.table_epoch = cache.table_epoch
 
 
 class SharedPagedKVCache(PagedKVCache):
@@ -88,7 +92,12 @@ class SharedPagedKVCache(PagedKVCache):
         w.require(self.records is not None, "shared cache: INT3 or INT5 block records, hq / h <= 8")
         self.page_refs = torch.zeros(pages, dtype=torch.int32, device=self.device)
         self.page_refs[0] = 1
+        self.table_epoch = 0  # counts the calls that may have assigned pages
+        self.replayed = False  # a graph's replays assign pages too, without the host
         self.reserve()
+
+    def _capturing(self):
+        return L.capturing(self.device.index)
 
     # ------------------------------------------------------------ pages
     def _seqs(self, seqs, what):
@@ -103,6 +112,8 @@ class SharedPagedKVCache(PagedKVCache):
         """Pages for the next ``ahead`` blocks of every sequence, or of sequence ``seqs``."""
         rows = slice(None) if seqs is None else slice(seqs, seqs + 1)
         P.reserve_pages(self.block_table[rows], self.n_blocks[rows], self.page_refs, ahead, self.status)
+        self.table_epoch += 1
+        self.replayed = self.replayed or self._capturing()
 
     def fork(self, src, dst):
         """Sequences ``dst`` become copies of sequence(s) ``src`` (one for all, or one each): the
@@ -197,12 +208,10 @@ class SharedPagedKVCache(PagedKVCache):
         w.require(all(groups) and len(set(flat)) == len(flat), "share: disjoint groups of sequences")
         return SharedPrefix(self, groups)
 
-    def _after_seal(self, plan=None):
+    def _after_seal(self):
         # a captured step replays with other counters: it always looks for pages
-        if torch.cuda.is_current_stream_capturing() or not self.host_tail.all():
+        if not self.host_tail.all() or self._capturing():
             self.reserve()
-            if plan is not None:
-                plan.refresh(self)
 
     def step(self, q, k_new, v_new, out=None, attn_event=None):
         o = super().step(q, k_new, v_new, out=out, attn_event=attn_event)
@@ -220,6 +229,8 @@ class SharedPagedKVCache(PagedKVCache):
         Prefix blocks are K- and V-rounded to the cache dtype as the bridge rounds them; own
         blocks follow ``restore_rounding``."""
         o = self.out if out is None else out
+        if plan.table_epoch != self.table_epoch or self.replayed or self._capturing():
+            plan.refresh(self)
         torch.sub(self.n_blocks, plan.first, out=plan.own_blocks)
         decode_attention(
             q, self.k_pool, self.v_pool, h=self.h, bits=self.bits, blk_stride_head=self.pages, blk_stride_page=1,
@@ -232,7 +243,7 @@ class SharedPagedKVCache(PagedKVCache):
                          row_index=plan.row_index, max_rows=plan.max_rows, o_part=plan.o_part,
                          lse_part=plan.lse_part, out=o, lse=plan.lse, status=self.status, ws=plan.ws)
         self.seal(1)
-        self._after_seal(plan)
+        self._after_seal()
         return o
 
     def check(self):

@@ -140,3 +140,90 @@ def test_shared_prompt_decoder(prompt):
     b.check()
     for c in b.caches:
         refs_hold(c)
+
+
+def pair(batch, prompt, groups, max_blocks=8, hq=4, dtype=torch.float16):
+    """A shared cache whose sequences are forks of one prompt, a plain cache holding the prompt per
+    sequence, and the plans of ``groups``."""
+    from nsn_b200.paged import PagedKVCache
+    from nsn_b200.shared import SharedPagedKVCache
+    h = 2
+    k, v = rows(prompt, h, 1, dtype)
+    plain = PagedKVCache(batch, h, max_blocks, dtype=dtype, hq=hq)
+    for b in range(batch):
+        plain.prefill(b, k, v)
+    shared = SharedPagedKVCache(batch, h, max_blocks, max_blocks * batch + 1, dtype=dtype, hq=hq)
+    shared.prefill(0, k, v)
+    shared.fork(0, range(1, batch))
+    return plain, shared, [shared.share(g) for g in groups]
+
+
+def agree(got, want, unit=2.0 ** -10):
+    """As test_forked_sequences_decode_like_separate_ones: 4 units of dtype."""
+    assert float((got.float() - want.float()).abs().max()) <= 4 * unit * max(1.0, float(want.float().abs().max()))
+
+
+@pytest.mark.parametrize("host", [False, True])
+def test_a_plan_follows_plain_steps(host):
+    """Plain steps seal blocks into pages that the plan was made before."""
+    plain, shared, (plan,) = pair(3, 200, [[[0, 1, 2]]])
+    for i in range(150):
+        q, kn, vn = token(3, 4, 2, i)
+        want = plain.step(q, kn, vn)
+        if host:
+            packed = torch.cat([x.reshape(-1) for x in (q, kn, vn)]).cpu().pin_memory()
+            out, done = torch.empty(3 * 4 * 128, dtype=q.dtype).pin_memory(), torch.cuda.Event()
+            shared.step_host(packed, out, done)
+            done.synchronize()
+        else:
+            shared.step(q, kn, vn)
+    q, kn, vn = token(3, 4, 2, 999)
+    agree(shared.step_shared(plan, q, kn, vn), plain.step(q, kn, vn))
+    refs_hold(shared)
+
+
+def test_two_plans_take_turns():
+    """Two plans of one cache on alternate steps: every second plan's steps never seal."""
+    plain, shared, plans = pair(4, 130, [[[0, 1, 2, 3]], [[0, 1], [2, 3]]])
+    for i in range(260):
+        q, kn, vn = token(4, 4, 2, i)
+        agree(shared.step_shared(plans[i % 2], q, kn, vn), plain.step(q, kn, vn))
+    refs_hold(shared)
+
+
+def test_a_plan_follows_extend():
+    """A sequence outside the batch's rhythm: more blocks appended behind its prefix."""
+    plain, shared, (plan,) = pair(2, 128, [[[0, 1]]])
+    k, v = rows(64 * 3, 2, 9)
+    shared.extend(1, k, v)
+    k0, v0 = rows(128, 2, 1)
+    plain.prefill(1, torch.cat([k0, k], 1), torch.cat([v0, v], 1))
+    q, kn, vn = token(2, 4, 2, 5)
+    agree(shared.step_shared(plan, q, kn, vn), plain.step(q, kn, vn))
+
+
+def test_a_captured_shared_step_among_eager_ones():
+    """Replays and eager steps of both kinds in turn: each finds the pages that the other took."""
+    plain, shared, (plan,) = pair(3, 70, [[[0, 1, 2]]])
+    q, kn, vn = token(3, 4, 2, 0)
+    out = torch.empty_like(q)
+    snap = shared.host_blocks.copy(), shared.host_tail.copy()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        shared.step_shared(plan, q, kn, vn, out=out)
+    shared.host_blocks[:], shared.host_tail[:] = snap
+    for i in range(300):
+        for x, y in zip((q, kn, vn), token(3, 4, 2, i)):
+            x.copy_(y)
+        want = plain.step(q, kn, vn)
+        if 60 <= i < 200 or i >= 280:  # 140 plain steps, then replays again, then shared steps
+            agree(shared.step(q, kn, vn) if i < 200 else shared.step_shared(plan, q, kn, vn), want)
+        else:
+            graph.replay()
+            agree(out, want)
+            shared.host_blocks[:] = shared.n_blocks.cpu().numpy()
+            shared.host_tail[:] = shared.tail_len.cpu().numpy()
+    refs_hold(shared)
+    del graph
+
