@@ -14,6 +14,8 @@ through caches of its own (experiments/ac08/source/loop_kv_ac08_attention.py:46-
 """
 from __future__ import annotations
 
+import weakref
+
 import numpy as np
 import torch
 
@@ -29,13 +31,14 @@ from .prompt import prompt_attention
 
 class SharedPrefix:
     """Which sequences of a cache share which leading pages, laid out for its step_shared
-    (made by SharedPagedKVCache.share; valid until a fork, free, prefill, import or compaction).
+    (made by SharedPagedKVCache.share; valid until a fork, free, prefill, import or compaction of it: step_shared refuses it then).
 
     ``own_table`` is a copy of the block table's entries behind the prefixes; step_shared brings it
     up to date when pages were assigned since (by any step, a seal, extend or reserve)."""
 
     def __init__(self, cache, groups):
         batch, dev = cache.batch, cache.device
+        self.cache, self.held = weakref.ref(cache), cache.held
         table = cache.block_table.cpu().numpy()  # the one host read, when the plan is made
         first, n_pages, order, offsets = np.zeros(batch, np.int64), [], [], [0]
         for seqs in groups:
@@ -93,6 +96,7 @@ class SharedPagedKVCache(PagedKVCache):
         self.page_refs = torch.zeros(pages, dtype=torch.int32, device=self.device)
         self.page_refs[0] = 1
         self.table_epoch = 0  # counts the calls that may have assigned pages
+        self.held = 0  # counts the calls that change what sequences hold other than by appending to them
         self.replayed = False  # a graph's replays assign pages too, without the host
         self.reserve()
 
@@ -129,6 +133,7 @@ class SharedPagedKVCache(PagedKVCache):
                          self._dev(src), self._dev(dst), self.status)
         self.host_blocks[dst] = self.host_blocks[src]
         self.host_tail[dst] = self.host_tail[src]
+        self.held += 1
         self.reserve()
 
     def free(self, seqs):
@@ -139,10 +144,13 @@ class SharedPagedKVCache(PagedKVCache):
         P.free_sequences(self.block_table, self.n_blocks, self.tail_len, self.page_refs, self._dev(seqs), self.status)
         self.host_blocks[seqs] = 0
         self.host_tail[seqs] = 0
+        self.held += 1
         self.reserve()
 
     def compact(self) -> torch.Tensor:
         """Bring the pages in use to the pool's front; returns their number (device int32 [1])."""
+        self.held += 1
+        self.table_epoch += 1
         return P.compact_pages([self.records, self.k_pool["norm"], self.v_pool["norm"]], self.block_table,
                                self.page_refs, table_out=self.block_table, refs_out=self.page_refs,
                                status=self.status)[2]
@@ -227,7 +235,9 @@ class SharedPagedKVCache(PagedKVCache):
         """``step`` with the plan's prefixes attended to once: append (k_new, v_new)
         [batch, h, 128], attend with q [batch, hq, 128] over prefix, own blocks and tail, seal.
         Prefix blocks are K- and V-rounded to the cache dtype as the bridge rounds them; own
-        blocks follow ``restore_rounding``."""
+        blocks follow ``restore_rounding``.  A graph that captured this call ends with its plan."""
+        w.require(plan.cache() is self and plan.held == self.held,
+                  "step_shared plan: of this cache, and made after its last fork, free, prefill, import and compaction")
         o = self.out if out is None else out
         if plan.table_epoch != self.table_epoch or self.replayed or self._capturing():
             plan.refresh(self)

@@ -227,3 +227,22 @@ def test_a_captured_shared_step_among_eager_ones():
     refs_hold(shared)
     del graph
 
+
+
+def test_a_plan_ends_with_what_its_sequences_held():
+    from nsn_b200 import ContractError
+    from nsn_b200.shared import SharedPagedKVCache
+    args = token(3, 4, 2, 0)
+    for change in (lambda c: c.free([2]), lambda c: c.fork(0, [1]), lambda c: c.prefill(1, *rows(200, 2, 4)),
+                   lambda c: c.compact(), lambda c: c.load_bytes(1, c.to_bytes(0))):
+        _, shared, (plan,) = pair(3, 200, [[[0, 1, 2]]])
+        shared.step_shared(plan, *args)
+        change(shared)
+        before = shared.lengths()
+        with pytest.raises(ContractError):
+            shared.step_shared(plan, *args)
+        assert torch.equal(shared.lengths(), before)
+        shared.step_shared(shared.share([[0, 1, 2]]), *args)
+    _, other, _ = pair(3, 200, [])
+    with pytest.raises(ContractError):  # a plan of another cache
+        other.step_shared(shared.share([[0, 1, 2]]), *args)
