@@ -221,6 +221,10 @@ class SharedPagedKVCache(PagedKVCache):
         if not self.host_tail.all() or self._capturing():
             self.reserve()
 
+    def seal(self, pending_append: int = 1):
+        super().seal(pending_append)
+        self._after_seal()
+
     def step(self, q, k_new, v_new, out=None, attn_event=None):
         o = super().step(q, k_new, v_new, out=out, attn_event=attn_event)
         self._after_seal()
@@ -253,7 +257,6 @@ class SharedPagedKVCache(PagedKVCache):
                          row_index=plan.row_index, max_rows=plan.max_rows, o_part=plan.o_part,
                          lse_part=plan.lse_part, out=o, lse=plan.lse, status=self.status, ws=plan.ws)
         self.seal(1)
-        self._after_seal()
         return o
 
     def check(self):

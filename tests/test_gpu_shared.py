@@ -246,3 +246,17 @@ def test_a_plan_ends_with_what_its_sequences_held():
     _, other, _ = pair(3, 200, [])
     with pytest.raises(ContractError):  # a plan of another cache
         other.step_shared(shared.share([[0, 1, 2]]), *args)
+
+
+def test_attend_and_seal_take_pages_too():
+    """The pair that step runs in one call, over several seals, against an ordinary cache."""
+    plain, shared, _ = pair(3, 70, [])
+    for i in range(200):
+        args = token(3, 4, 2, i)
+        want, got = plain.attend(*args).clone(), shared.attend(*args)
+        plain.seal(1)
+        shared.seal(1)
+        assert torch.equal(got, want), i
+    refs_hold(shared)
+    assert [shared.to_bytes(b) for b in range(3)] == [plain.to_bytes(b) for b in range(3)]
+    shared.check()
