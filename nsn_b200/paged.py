@@ -322,12 +322,9 @@ class PagedKVCache:
         return (group(self.k_pool), self.k_tail[b, :, :t].unsqueeze(0).contiguous(), group(self.v_pool),
                 self.v_tail[b, :, :t].unsqueeze(0).contiguous())
 
-    def import_groups(self, b: int, kg, kt, vg, vt):
-        """Load sequence b from the reference's layout; headers are verified.
-
-        A tail of 64 tokens or more (the reference's PackedCache keeps 64..127) is sealed
-        into further blocks, so the cache's seal-at-64 invariant holds afterwards.
-        """
+    def _import_sizes(self, kg, kt, vg, vt):
+        """Checks of a sequence in the reference's layout; (sealed blocks, blocks its tail fills,
+        tokens left over)."""
         h = self.h
         n = 0 if kg is None else kg["codes"].shape[2]
         w.require((kg is None) == (vg is None) and kt.shape == vt.shape and tuple(kt.shape[:2]) == (1, h)
@@ -339,6 +336,16 @@ class PagedKVCache:
         t = kt.shape[2]
         extra, rest = t // w.BLOCK, t % w.BLOCK
         w.require(n + extra <= self.max_blocks, "import exceeds max_blocks")
+        return n, extra, rest
+
+    def import_groups(self, b: int, kg, kt, vg, vt):
+        """Load sequence b from the reference's layout; headers are verified.
+
+        A tail of 64 tokens or more (the reference's PackedCache keeps 64..127) is sealed
+        into further blocks, so the cache's seal-at-64 invariant holds afterwards.
+        """
+        h = self.h
+        n, extra, rest = self._import_sizes(kg, kt, vg, vt)
         pages = self.block_table[b, :n].long()
         for g, pool in ((kg, self.k_pool), (vg, self.v_pool)):
             if g is None:

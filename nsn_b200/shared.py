@@ -195,9 +195,7 @@ class SharedPagedKVCache(PagedKVCache):
 
     def import_groups(self, b: int, kg, kt, vg, vt):
         """Load sequence b from the reference's layout (see PagedKVCache.import_groups)."""
-        h, n = self.h, 0 if kg is None else kg["codes"].shape[2]
-        w.require((kg is None) == (vg is None) and kt.shape == vt.shape and tuple(kt.shape[:2]) == (1, h)
-                  and kt.shape[-1] == w.DIM and n <= self.max_blocks, "import layout")
+        n = self._import_sizes(kg, kt, vg, vt)[0]
         self.free([b])
         self.reserve(b, min(n + 1, self.max_blocks))
         if n:

@@ -260,3 +260,24 @@ def test_attend_and_seal_take_pages_too():
     refs_hold(shared)
     assert [shared.to_bytes(b) for b in range(3)] == [plain.to_bytes(b) for b in range(3)]
     shared.check()
+
+
+def test_import_checks_what_it_loads():
+    """Groups of another head count, wrong headers, missing blocks: refused as by PagedKVCache."""
+    from nsn_b200 import ContractError
+    from nsn_b200.shared import SharedPagedKVCache
+    c = SharedPagedKVCache(2, 2, 6, 20, hq=4)
+    one = SharedPagedKVCache(2, 1, 6, 20, hq=2)
+    c.prefill(0, *rows(64 * 2 + 5, 2, 0))
+    one.prefill(0, *rows(64 * 2 + 5, 1, 0))
+    kg, kt, vg, vt = c.export_groups(0)
+    kg1, _, vg1, _ = one.export_groups(0)
+    wrong = dict(kg, headers=kg["headers"].clone())
+    wrong["headers"][0, 1, 0, 8] ^= 1
+    short = {**vg, "codes": vg["codes"][:, :, :1]}
+    for bad in ((kg1, kt, vg1, vt), (wrong, kt, vg, vt), (kg, kt, dict(vg, headers=wrong["headers"]), vt),
+                (kg, kt, short, vt)):
+        with pytest.raises(ContractError):
+            c.import_groups(1, *bad)
+    c.import_groups(1, kg, kt, vg, vt)
+    assert c.to_bytes(1) == c.to_bytes(0)
