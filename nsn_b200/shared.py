@@ -162,10 +162,14 @@ class SharedPagedKVCache(PagedKVCache):
         self.k_pool["norm"][:, pages] = k_norm
         self.v_pool["norm"][:, pages] = v_norm
 
+    def _native(self, k, v, what):
+        w.require(k.shape == v.shape and k.ndim == 3 and k.shape[0] == self.h and k.shape[2] == w.DIM, f"{what} shape")
+        w.require(k.shape[1] < w.BLOCK or k.device == v.device == self.device, f"{what}: K and V on the cache's device")
+
     def extend(self, b: int, k: torch.Tensor, v: torch.Tensor):
         """Append native K/V [h, T, 128] to sequence b, whose tail is empty: T // 64 blocks are
         sealed, T % 64 tokens become the tail."""
-        w.require(k.shape == v.shape and k.ndim == 3 and k.shape[0] == self.h and k.shape[2] == w.DIM, "extend shape")
+        self._native(k, v, "extend")
         w.require(self.host_tail[b] == 0, "extend: the sequence's tail is not empty")
         n, t = k.shape[1] // w.BLOCK, k.shape[1] % w.BLOCK
         w.require(self.host_blocks[b] + n <= self.max_blocks, "extend exceeds max_blocks")
@@ -190,20 +194,24 @@ class SharedPagedKVCache(PagedKVCache):
 
     def prefill(self, b: int, k: torch.Tensor, v: torch.Tensor):
         """Load sequence b from native K/V [h, T, 128] (what it held is given back)."""
+        self._native(k, v, "prefill")
+        w.require(k.shape[1] // w.BLOCK <= self.max_blocks, "prefill exceeds max_blocks")
         self.free([b])
         self.extend(b, k, v)
 
     def import_groups(self, b: int, kg, kt, vg, vt):
         """Load sequence b from the reference's layout (see PagedKVCache.import_groups)."""
         n = self._import_sizes(kg, kt, vg, vt)[0]
-        self.free([b])
-        self.reserve(b, min(n + 1, self.max_blocks))
         if n:
             dev = lambda g: dict(g, codes=g["codes"].to(self.device), metas=tuple(m.to(self.device) for m in g["metas"]))
             records, kp, vp = group_record_pools(dev(kg), dev(vg), self.bits)
+        kt, vt = (x[0].to(self.device, self.dtype) for x in (kt, vt))
+        self.free([b])  # nothing is refused from here on
+        self.reserve(b, min(n + 1, self.max_blocks))
+        if n:
             self._put(b, n, records, kp["norm"], vp["norm"])
         self._advance(b, n, 0)
-        self.extend(b, kt[0].to(self.device, self.dtype), vt[0].to(self.device, self.dtype))
+        self.extend(b, kt, vt)
 
     # ------------------------------------------------------------ decode
     def share(self, groups) -> SharedPrefix:

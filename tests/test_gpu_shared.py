@@ -281,3 +281,24 @@ def test_import_checks_what_it_loads():
             c.import_groups(1, *bad)
     c.import_groups(1, kg, kt, vg, vt)
     assert c.to_bytes(1) == c.to_bytes(0)
+
+
+def test_a_refused_load_leaves_the_sequence():
+    from nsn_b200 import ContractError
+    from nsn_b200.shared import SharedPagedKVCache
+    c = SharedPagedKVCache(2, 2, 4, 20, hq=4)
+    big = SharedPagedKVCache(1, 2, 6, 20, hq=4)
+    c.prefill(1, *rows(64 * 2 + 5, 2, 0))
+    big.prefill(0, *rows(64 * 4 + 1, 2, 1))
+    kg, kt, vg, vt = big.export_groups(0)
+    before = c.to_bytes(1)
+    k, v = rows(100, 2, 3)
+    for bad in (lambda: c.prefill(1, *rows(64 * 5, 2, 0)), lambda: c.prefill(1, k, v[:, :99]),
+                lambda: c.prefill(1, k[:1], v[:1]), lambda: c.prefill(1, k[..., :64], v[..., :64]),
+                lambda: c.prefill(1, k.cpu(), v.cpu()),
+                lambda: c.import_groups(1, kg, torch.cat([kt] * 64, 2), vg, torch.cat([vt] * 64, 2)),
+                lambda: c.import_groups(1, kg, kt, None, vt), lambda: c.import_groups(1, kg, kt[:, :1], vg, vt[:, :1])):
+        with pytest.raises(ContractError):
+            bad()
+        assert c.to_bytes(1) == before
+    refs_hold(c)
