@@ -488,7 +488,7 @@ int nsnkv_k1c_scores(int recipe, int64_t batch, int n_q, int n_kv, int64_t token
  *   tokens       rows of q, k, v and out; cu_seqlens int32 [seqs + 1] on the device, ascending,
  *                within [0, tokens] (values outside are clamped); rows that no sequence covers
  *                are not written
- *   longest      the longest sequence as far as the caller knows: it sizes the grid only
+ *   longest      the longest sequence as far as the caller knows (0: not known): it sizes the grid only
  *   q, k, v      token t of head j starts at element t * tok + j * head of its own strides
  *                (views of one fused projection are fine); 128 contiguous channels per head,
  *                strides multiples of 8 elements, pointers 16-byte aligned; dtype F16 or BF16

@@ -202,7 +202,7 @@ extern "C" int nsnkv_prompt_attn(int64_t tokens, int32_t seqs, int64_t longest, 
   if (tokens < 0 || seqs < 0 || seqs > 65535 || longest < 0 || hq <= 0 || h <= 0 || hq % h || hq > 65535)
     return NSNKV_ERR_ARG;
   if (dtype != NSNKV_F16 && dtype != NSNKV_BF16) return NSNKV_ERR_ARG;
-  if (tokens == 0 || seqs == 0 || longest == 0) return NSNKV_OK;
+  if (tokens == 0 || seqs == 0) return NSNKV_OK;
   if (!q || !k || !v || !cu_seqlens || !out || !aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out))
     return NSNKV_ERR_ARG;
   for (int64_t s : {q_tok, q_head, k_tok, k_head, v_tok, v_head})
@@ -210,7 +210,7 @@ extern "C" int nsnkv_prompt_attn(int64_t tokens, int32_t seqs, int64_t longest, 
   PromptArgs a{q, k, v, out, lse, cu_seqlens, tokens, q_tok, q_head, k_tok, k_head, v_tok, v_head, seqs, hq, h,
                causal != 0, status};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (longest > tokens) longest = tokens;
+  if (longest == 0 || longest > tokens) longest = tokens;  // 0: not known
   if (tokens > INT32_MAX || (tokens / 256 + seqs) * hq > INT32_MAX) return NSNKV_ERR_TOO_LARGE;
   // The tensor-core kernel from 65 rows on: 16 sequences of 64 tokens, GQA 32:8, take 18.3 us here and
   // 19.9 us there, of 128 tokens 33.0 and 21.8 us, of 256 tokens 72.6 and 36.2 us.  Its stores are

@@ -19,8 +19,8 @@ def prompt_attention(q, k, v, cu_seqlens, max_seqlen, *, causal=True, out=None, 
     cu_seqlens[s] .. cu_seqlens[s + 1] (int32 [seqs + 1] on the GPU, ascending from 0 to T).
 
     q, k and v may be views with any token and head strides that are multiples of 8 elements
-    (slices of one fused projection).  ``max_seqlen``: the longest sequence, as far as known:
-    it sizes the launch, not the result.  Returns (out [T, hq, 128] in the inputs' dtype,
+    (slices of one fused projection).  ``max_seqlen``: the longest sequence, as far as known
+    (0: not known): it sizes the launch, not the result.  Returns (out [T, hq, 128] in the inputs' dtype,
     lse [T, hq] fp32); rows that no sequence covers are not written.  ``status`` (int32 [1]):
     NSNKV_ST_OUTPUT_NONFINITE is OR-ed in when an output is not finite.  No host sync.
     """

@@ -248,3 +248,13 @@ def test_a_row_without_a_finite_score_is_nan(lens, where):
     out, lse = prompt_attention(q, k, v, cu, max(lens))
     assert bool(out[bad].isnan().all()) and bool(lse[bad].isnan().all())
     check(out, lse, ref, ~bad)
+
+
+@pytest.mark.parametrize("lens", [[30], [513, 20]], ids=str)
+def test_an_unknown_longest_sequence(lens):
+    """max_seqlen 0 is not known: the whole call is computed."""
+    from nsn_b200.prompt import prompt_attention
+    q, k, v, cu = make(lens, 4, 2, torch.float16)
+    out, lse = torch.full_like(q, 7.0), torch.full((sum(lens), 4), 7.0, device="cuda")
+    prompt_attention(q, k, v, cu, 0, out=out, lse=lse)
+    check(out, lse, reference(q, k, v, lens))
