@@ -11,12 +11,13 @@
 // row tile both softmax teams work on it, on alternate blocks, and join their halves at the end.
 //
 // What bounds it is the restore: 16384 values a block, about four instructions each, whatever
-// the rows.  A code is moved to bits 13..22 of a word and one AND-OR with the bits of 1.0f makes
-// it the float 1 + code 2^(p - 23), p its bit; with a = scale 2^(23 - p) and b = min - a, the
-// direction min + scale * code is one fused multiply-add a * (1 + code 2^(p - 23)) + b.  That is
-// the separately rounded min + scale * code wherever b is exact, i.e. wherever min's last bit is
-// not below 2^-24 of a (true of unit directions: min and scale within a few powers of two);
-// elsewhere it is within 2^-24 a of it.  a and b are laid out once per block and channel.
+// the rows.  A code is moved to bits 13..22 of a word, and one AND leaves it the subnormal float
+// code 2^(p - 149), p its bit (fused multiply-adds take subnormals at full rate).  With
+// a = scale 2^(117 - p) and b = min 2^-32, both exact, one fused multiply-add gives
+// 2^-32 (min + scale * code): scale * code has at most 16 bits, so this is the sum rounded once,
+// as restore_group rounds it, and no result is subnormal (min and scale are multiples of 2^-24).
+// alpha 2^32 takes the factor back in the product (alpha is at most 65504 / 1e-12).  a and b are
+// laid out once per block and channel.
 //
 // Measured: 64 rows over 8192 INT3 tokens, GQA 32:8: 35.4 us with the merge (eight blocks per CTA at
 // 2400 cycles between a start of 9 k cycles and 8 k of writing partial rows); 8 rows over 131008
@@ -80,27 +81,21 @@ __device__ __forceinline__ void windows(const uint32_t (&s)[(BITS + 1) / 2], uin
 
 template <int I> struct Int { static constexpr int value = I; };
 
-// (x & mask) | one: one logic instruction, with the bits of 1.0f in a register.
-template <uint32_t MASK>
-__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t one) {
-  uint32_t d;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(x), "n"(MASK), "r"(one));
-  return d;
-}
+constexpr float kDown = 0x1p-32f, kUp = 0x1p32f;  // see above: directions are held 2^-32 times as large
 
 // Sixteen codes of a stream -> 16 values of T (channels 16 c ..) as two 16-byte chunks.
 template <int BITS, typename T>
 __device__ __forceinline__ void values16(const uint32_t (&s)[(BITS + 1) / 2], const float4 (&ab)[8], float alpha,
-                                         uint32_t one, uint4 (&out)[2]) {
+                                         uint4 (&out)[2]) {
   using W = Window<BITS>;
   uint32_t x[W::kCount], r[8];
   windows<BITS>(s, x);
-  const float2 al = make_float2(alpha, alpha);
+  const float2 al = make_float2(alpha * kUp, alpha * kUp);
   constexpr uint32_t kMask = (1u << BITS) - 1u;
   auto pair = [&](auto I) {
     constexpr int i = decltype(I)::value;
-    const float2 v = make_float2(__uint_as_float(and_or<kMask << W::bit(2 * i)>(x[2 * i / W::kPer], one)),
-                                 __uint_as_float(and_or<kMask << W::bit(2 * i + 1)>(x[(2 * i + 1) / W::kPer], one)));
+    const float2 v = make_float2(__uint_as_float(x[2 * i / W::kPer] & kMask << W::bit(2 * i)),
+                                 __uint_as_float(x[(2 * i + 1) / W::kPer] & kMask << W::bit(2 * i + 1)));
     const float2 d = tc::fma2(make_float2(ab[i].x, ab[i].y), v, make_float2(ab[i].z, ab[i].w));
     const float2 y = tc::mul2(d, al);
     r[i] = rr::round2<T>(y.x, y.y);
@@ -382,9 +377,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
       // and 2 r8 + 32 e + 1 (whose swizzle exchanges the two chunks)
       const int k_src = (r8 * 4 * BITS + (g16 >> 1) * BITS) * 4, v_src = R::kHalf + (r8 * 8 + g16) * BITS * 4;
       const int k_dst = chunk_at(r8, 2 * g16), v_dst = kRowsBytes + chunk_at(2 * r8, 2 * g16);
-      const float mul = __int_as_float((127 + 23 - Window<BITS>::bit(ch & 15)) << 23);
-      uint32_t one;
-      asm volatile("mov.u32 %0, 0x3F800000;" : "=r"(one));  // kept in a register
+      const float mul = __int_as_float((127 + 117 - Window<BITS>::bit(ch & 15)) << 23);
       const int mine = team ^ (blocks & 1);                 // the first block of this chunk that is the team's
       uint32_t slot = (blocks + mine) % kR, raw_par = (blocks + mine) / kR & 1;
       uint32_t stage = (blocks + mine) % kStages, par = (blocks + mine) / kStages & 1;
@@ -396,11 +389,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
 #pragma unroll
         for (int x = 0; x < 2; ++x) {  // K, V; channel pairs as (a, a, b, b)
           const uint16_t *half = reinterpret_cast<const uint16_t *>(rec + x * R::kHalf + R::kMin) + ch;
-          const float mn = half_bits_to_f(half[0]), sc = half_bits_to_f(half[128]), p = sc * mul, y = mn - p;
-          bad |= !isfinite(y);
+          const float mn = half_bits_to_f(half[0]), sc = half_bits_to_f(half[128]);
+          bad |= !isfinite(mn + sc);
           float *dst = reinterpret_cast<float *>(&S.ab[team][x][ch & ~1]) + (ch & 1);
-          dst[0] = p;
-          dst[2] = y;
+          dst[0] = sc * mul;
+          dst[2] = mn * kDown;
         }
         tc::bar_named(1 + team, 128);
         tc::spin(&S.empty[stage], par ^ 1, &S.failed, a.status);
@@ -421,7 +414,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
 #pragma unroll
           for (int i = 0; i < (BITS + 1) / 2; ++i)
             st[i] = __byte_perm(wd[2 * i], 2 * i + 1 < BITS ? wd[2 * i + 1] : 0u, sel);
-          values16<BITS, T>(st, ab, alpha, one, out);
+          values16<BITS, T>(st, ab, alpha, out);
           *reinterpret_cast<uint4 *>(rows + k_dst + e * 16 * 128) = out[0];
           *reinterpret_cast<uint4 *>(rows + (k_dst ^ 16) + e * 16 * 128) = out[1];
         }
@@ -440,7 +433,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefix_tc_kernel(const __grid_con
 #pragma unroll
             for (int i = 0; i < (BITS + 1) / 2; ++i)
               st[i] = __byte_perm(wd[2 * i], 2 * i + 1 < BITS ? wd[2 * i + 1] : 0u, y ? 0x7632u : 0x5410u);
-            values16<BITS, T>(st, ab, y ? alpha.y : alpha.x, one, out);
+            values16<BITS, T>(st, ab, y ? alpha.y : alpha.x, out);
             *reinterpret_cast<uint4 *>(dst + (v_dst ^ (16 * y)) + y * 128) = out[0];
             *reinterpret_cast<uint4 *>(dst + (v_dst ^ (16 * (1 - y))) + y * 128) = out[1];
           }

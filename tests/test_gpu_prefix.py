@@ -322,3 +322,43 @@ def test_a_nan_part_is_not_dropped(blocks):
     assert bool(out[2:4].isnan().all()) and bool(lse[2:4].isnan().all())
     keep = torch.tensor([0, 1, 4], device="cuda")
     check((out[keep], lse[keep]), [t[keep] for t in ref])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("bits", [3, 5])
+def test_rows_are_restored_bit_for_bit(bits, dtype):
+    """K and V rows equal alpha (min + scale code), each step rounded to fp32 and the result to
+    dtype, for channels whose minimum is small beside their scale (one-signed channels) too.
+
+    Page t holds random codes and a K factor in token t only, so that a row of group t with a
+    large q sees that token alone.  Channel 0 of K is the factor itself: with q = 8 along it the
+    score is some 1000, p is 1 within 2^-13 and the output the token's V row.  With q along
+    channel c the log-sum-exp is q K[c] / sqrt(128) within 2^-21 of its size, which names K[c]
+    among the values of dtype (2^-11 apart and more)."""
+    from nsn_b200 import paged
+    from nsn_b200.prefix import prefix_attention
+    g = torch.Generator(device="cuda").manual_seed(bits)
+    rec, kp, vp = paged.block_record_pools(1, 64, bits, "cuda")
+    mins = torch.tensor([1.0, 0.1, 1e-3, 6e-8, 3e-2, 0.02, 1e-4, 5e-3], device="cuda").repeat(16)
+    steps = torch.tensor([0.1, 0.0123, 0.777, 0.05, 0.1, 0.3], device="cuda").repeat(22)[:128]
+    for p in (kp, vp):
+        p["codes"].copy_(torch.randint(0, 256, p["codes"].shape, generator=g, dtype=torch.uint8, device="cuda"))
+        p["min"].copy_(mins.half())
+        p["scale"].copy_(steps.half())
+    vp["min"][..., 1::3] *= -1
+    kp["scale"][..., 0] = 0
+    t, c = torch.arange(64, device="cuda"), torch.arange(128, device="cuda")
+    kp["alpha"].zero_()
+    kp["alpha"][0, t, t] = 1024 * (1 + torch.rand(64, generator=g, device="cuda"))
+    vp["alpha"].copy_(torch.rand(vp["alpha"].shape, generator=g, device="cuda") * 20 + 0.1)
+    k, v = rows_of(kp, bits, dtype)[0, t, t], rows_of(vp, bits, dtype)[0, t, t]  # [64, 128]
+    dev = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    size = torch.where(c == 0, 8.0, 32768.0)
+    q = torch.diag(size).to(dtype).repeat(64, 1)[:, None].contiguous()  # row 128 t + c: along channel c
+    out, lse = prefix_attention(q, rec, dev(list(range(64)))[:, None], dev([1] * 64), bits=bits,
+                                row_offsets=dev([128 * i for i in range(65)]), max_rows=128)
+    out, lse = out.reshape(64, 128, 128), lse.reshape(64, 128)
+    assert torch.equal(out[:, 0], v)
+    known = k.float() * size / math.sqrt(128) > 150  # the other 63 tokens' p are 0
+    assert float(known.float().mean()) > 0.9
+    assert torch.equal((lse.double() * math.sqrt(128) / size).to(dtype)[known], k[known])
