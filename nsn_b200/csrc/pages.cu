@@ -23,8 +23,8 @@ struct ForkArgs {
 };
 
 __device__ __forceinline__ void drop_ref(int32_t *refs, int64_t pages, int32_t page, int32_t *status) {
-  if (page <= 0) return;
-  if (page < pages)
+  if (page == 0) return;
+  if (page > 0 && page < pages)
     atomicSub(refs + page, 1);
   else
     set_status(status, NSNKV_ST_PAGE);
@@ -44,9 +44,13 @@ __global__ void __launch_bounds__(128) fork_kernel(const ForkArgs a) {
     const int32_t n = min(max(a.n_blocks[s], 0), a.max_blocks);
     int32_t *from = a.table + s * a.table_stride, *to = a.table + d * a.table_stride;
     for (int i = tid; i < a.max_blocks; i += 128) {
-      const int32_t next = i < n ? from[i] : 0;
+      int32_t next = i < n ? from[i] : 0;
+      if (next < 0 || next >= a.pages) {  // names no page of the pool: not handed on
+        set_status(a.status, NSNKV_ST_PAGE);
+        next = 0;
+      }
       drop_ref(a.refs, a.pages, to[i], a.status);
-      if (next > 0 && next < a.pages) atomicAdd(a.refs + next, 1);
+      if (next > 0) atomicAdd(a.refs + next, 1);
       to[i] = next;
     }
     if (tid == 0) {

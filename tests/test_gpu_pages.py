@@ -183,3 +183,40 @@ def test_refusals():
         P.compact_pages([rec, rec[:, :12]], d["table"], d["refs"])
     with pytest.raises(ContractError):
         P.copy_pages([rec], one, two)
+
+
+def test_fork_drops_entries_outside_the_pool():
+    """A source entry that names no page of the pool is not handed on: 0 in the target, and a status."""
+    from nsn_b200.pages import fork_sequences
+    s = state(3, 6, 19, seed=1)
+    s["n"][0] = 5
+    s["table"][0, 1], s["table"][0, 3] = 19, -4
+    d = {k: dev(v) for k, v in s.items()}
+    st = torch.zeros(1, dtype=torch.int32, device="cuda")
+    fork_sequences(d["table"], d["n"], d["tl"], d["refs"], d["kt"], d["vt"], dev(np.int32([0])), dev(np.int32([2])),
+                   status=st)
+    for p in s["table"][2]:
+        s["refs"][p] -= p > 0
+    row = np.where(np.arange(6) < 5, s["table"][0], 0)
+    row[[1, 3]] = 0
+    for p in row:
+        s["refs"][p] += p > 0
+    s["table"][2], s["n"][2], s["tl"][2] = row, 5, s["tl"][0]
+    s["kt"][2, :, :s["tl"][0]], s["vt"][2, :, :s["tl"][0]] = s["kt"][0, :, :s["tl"][0]], s["vt"][0, :, :s["tl"][0]]
+    same(s, d)
+    assert int(st) == 128
+
+
+def test_free_reports_entries_outside_the_pool():
+    from nsn_b200.pages import free_sequences
+    for value in (13, -1):
+        s = state(3, 4, 13, seed=2)
+        s["table"][1, 3] = value
+        d = {k: dev(v) for k, v in s.items()}
+        st = torch.zeros(1, dtype=torch.int32, device="cuda")
+        free_sequences(d["table"], d["n"], d["tl"], d["refs"], dev(np.int32([1])), status=st)
+        for p in s["table"][1, :3]:
+            s["refs"][p] -= p > 0
+        s["table"][1] = s["n"][1] = s["tl"][1] = 0
+        same(s, d)
+        assert int(st) == 128
