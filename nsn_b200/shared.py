@@ -248,6 +248,8 @@ class SharedPagedKVCache(PagedKVCache):
         blocks follow ``restore_rounding``.  A graph that captured this call ends with its plan."""
         w.require(plan.cache() is self and plan.held == self.held,
                   "step_shared plan: of this cache, and made after its last fork, free, prefill, import and compaction")
+        if ((self.host_blocks >= self.max_blocks) & (self.host_tail + 1 >= w.BLOCK)).any():
+            L.check(L.ERR_TOO_LARGE, "step_shared")  # as step: the tail must keep a free row
         o = self.out if out is None else out
         if plan.table_epoch != self.table_epoch or self.replayed or self._capturing():
             plan.refresh(self)
@@ -268,7 +270,8 @@ class SharedPagedKVCache(PagedKVCache):
     def check(self):
         st = int(self.status.item())
         if st & (L.ST_CAPACITY | L.ST_PAGE):
-            raise w.ContractError("shared cache: the page pool is exhausted" if st & L.ST_CAPACITY
+            raise w.ContractError("shared cache: no page for a block (the pool is exhausted, or a replay went past "
+                                  "max_blocks)" if st & L.ST_CAPACITY
                                   else "shared cache: a page number outside the pool")
         super().check()
 

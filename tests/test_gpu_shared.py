@@ -302,3 +302,18 @@ def test_a_refused_load_leaves_the_sequence():
             bad()
         assert c.to_bytes(1) == before
     refs_hold(c)
+
+
+def test_a_full_sequence_refuses_the_shared_step():
+    """The step that would fill the last tail is refused before anything changes, as step's is."""
+    from nsn_b200._lib import NativeError
+    _, shared, (plan,) = pair(2, 64 * 3 + 60, [[[0, 1]]], max_blocks=3)
+    args = token(2, 4, 2, 0)
+    for _ in range(3):
+        shared.step_shared(plan, *args)
+    for call in (lambda: shared.step_shared(plan, *args), lambda: shared.step(*args)):
+        with pytest.raises(NativeError):
+            call()
+        assert shared.host_blocks.tolist() == [3, 3] and shared.host_tail.tolist() == [63, 63]
+        refs_hold(shared)
+    shared.check()
