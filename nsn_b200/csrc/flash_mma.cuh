@@ -46,6 +46,19 @@ template <> __device__ __forceinline__ uint32_t round_pair<__nv_bfloat16>(float 
   return *reinterpret_cast<const uint32_t *>(&p);
 }
 
+// acc + 0 * w per element of a packed pair: NaN once a w held NaN or an infinity, else 0.
+template <typename T> __device__ __forceinline__ uint32_t add_zero_times(uint32_t acc, uint32_t w);
+template <> __device__ __forceinline__ uint32_t add_zero_times<__half>(uint32_t acc, uint32_t w) {
+  const __half2 r = __hfma2(*reinterpret_cast<const __half2 *>(&w), __float2half2_rn(0.f),
+                            *reinterpret_cast<const __half2 *>(&acc));
+  return *reinterpret_cast<const uint32_t *>(&r);
+}
+template <> __device__ __forceinline__ uint32_t add_zero_times<__nv_bfloat16>(uint32_t acc, uint32_t w) {
+  const __nv_bfloat162 r = __hfma2(*reinterpret_cast<const __nv_bfloat162 *>(&w), __float2bfloat162_rn(0.f),
+                                   *reinterpret_cast<const __nv_bfloat162 *>(&acc));
+  return *reinterpret_cast<const uint32_t *>(&r);
+}
+
 // The state of a warp's 16 rows.  Lane (g = lane / 4, t = lane % 4) holds rows g and g + 8.
 struct Rows {
   uint32_t q[8][4];  // A fragments of Q, k-step ks: channels 16 ks ..

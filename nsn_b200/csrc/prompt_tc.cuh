@@ -536,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t o_at = tmem + (static_cast<uint32_t>(warp & 3) << 21) + 256 + 128 * t;
       const int64_t at = static_cast<int64_t>(it.begin + row) * a.hq + it.head;
       T *orow = static_cast<T *>(a.out) + at * kDim;
-      float2 check = make_float2(0.f, 0.f);  // 0 * y summed: NaN when an output is not finite
+      uint32_t check = 0;  // 0 * w summed: NaN when a rounded output is not finite
 #pragma unroll 1
       for (int i = 0; i < 4; ++i) {
         float o[32];
@@ -547,8 +547,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const float2 y = tc::mul2(make_float2(o[2 * e], o[2 * e + 1]), make_float2(inv, inv));
-          check = tc::fma2(y, make_float2(0.f, 0.f), check);
           w[e] = fm::round_pair<T>(y.x, y.y);
+          check = fm::add_zero_times<T>(check, w[e]);
         }
         if (row < it.len) {
           tc::store32(orow + 32 * i, w);
@@ -557,7 +557,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       tc::fence_before();  // O is read before the next item's first P is announced
       if (row < it.len) {
-        if (check.x + check.y != 0.f) atomicOr(&S.redo[t][k >> 5 & 31], 1u << (k & 31));
+        const float2 nan = Elem<T>::to_f2(check);
+        if (nan.x + nan.y != 0.f) atomicOr(&S.redo[t][k >> 5 & 31], 1u << (k & 31));
         if (a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * fm::kLn2;
       }
     }

@@ -258,3 +258,27 @@ def test_an_unknown_longest_sequence(lens):
     out, lse = torch.full_like(q, 7.0), torch.full((sum(lens), 4), 7.0, device="cuda")
     prompt_attention(q, k, v, cu, 0, out=out, lse=lse)
     check(out, lse, reference(q, k, v, lens))
+
+
+@pytest.mark.parametrize("T", [60, 200])
+def test_an_output_that_rounds_past_the_type_is_reported(T):
+    """V at fp16's largest value and probabilities that all round up: sum round(p) v / sum p is
+    above 65520, which is infinity in fp16; the status word has to say so.
+
+    Token 0's score is x above the others', x log2(e) = 1 - log2(1 + 5 2^-13): their p is
+    1/2 + 5 2^-14, between the midpoint 1/2 + 2^-12 of two fp16 values and the upper one."""
+    from nsn_b200.prompt import prompt_attention
+    x = (1 - math.log2(1 + 5 * 2.0 ** -13)) / 1.4426950408889634 * math.sqrt(128)  # q . (k_0 - k_j)
+    q = torch.zeros((T, 1, 128), dtype=torch.float16, device="cuda")
+    k = torch.zeros_like(q)
+    hi = float(torch.tensor(x, dtype=torch.float16))
+    lo = float(torch.tensor((x - hi) * 1024, dtype=torch.float16))  # x = hi + lo / 1024 within 2^-20
+    q[..., 0] = 1
+    q[..., 1] = 1 / 1024
+    k[0, 0, 0], k[0, 0, 1] = hi, lo
+    v = torch.full_like(q, 65504.0)
+    cu = torch.tensor([0, T], dtype=torch.int32, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out, _ = prompt_attention(q, k, v, cu, T, status=status)
+    assert bool(out[-1].isinf().all())  # the case is what it says
+    assert int(status) == 8
