@@ -28,10 +28,6 @@ def _ints(name, dev, *tensors):
         raise w.ContractError(f"{name}: int32 CUDA tensors on one device")
 
 
-def _p(t):
-    return None if t is None else t.data_ptr()
-
-
 def fork_sequences(block_table, n_blocks, tail_len, page_refs, k_tail, v_tail, src, dst, status=None):
     """Sequence dst[i] becomes a copy of sequence src[i]: it drops the pages it held, shares
     src's sealed pages and copies src's counters and tail rows.
@@ -54,7 +50,7 @@ def fork_sequences(block_table, n_blocks, tail_len, page_refs, k_tail, v_tail, s
     rc = L.call_on(index, L.load().nsnkv_fork_sequences, batch, h, page_refs.shape[0], block_table.data_ptr(),
                    block_table.stride(0), max_blocks, n_blocks.data_ptr(), tail_len.data_ptr(), page_refs.data_ptr(),
                    k_tail.data_ptr(), v_tail.data_ptr(), h * w.BLOCK, w.BLOCK, src.shape[0], src.data_ptr(),
-                   dst.data_ptr(), _p(status), L.raw_stream(index))
+                   dst.data_ptr(), w.status_ptr(status, dev), L.raw_stream(index))
     if rc:
         L.check(rc, "nsnkv_fork_sequences")
 
@@ -68,7 +64,7 @@ def free_sequences(block_table, n_blocks, tail_len, page_refs, seqs, status=None
     index = dev.index
     rc = L.call_on(index, L.load().nsnkv_free_sequences, batch, page_refs.shape[0], block_table.data_ptr(),
                    block_table.stride(0), max_blocks, n_blocks.data_ptr(), tail_len.data_ptr(), page_refs.data_ptr(),
-                   seqs.shape[0], seqs.data_ptr(), _p(status), L.raw_stream(index))
+                   seqs.shape[0], seqs.data_ptr(), w.status_ptr(status, dev), L.raw_stream(index))
     if rc:
         L.check(rc, "nsnkv_free_sequences")
 
@@ -83,8 +79,8 @@ def reserve_pages(block_table, n_blocks, page_refs, ahead=1, status=None):
         raise w.ContractError("reserve_pages tables: block_table [batch, max_blocks], n_blocks [batch]")
     index = dev.index
     rc = L.call_on(index, L.load().nsnkv_reserve_pages, batch, page_refs.shape[0], block_table.data_ptr(),
-                   block_table.stride(0), max_blocks, n_blocks.data_ptr(), page_refs.data_ptr(), int(ahead), _p(status),
-                   L.raw_stream(index))
+                   block_table.stride(0), max_blocks, n_blocks.data_ptr(), page_refs.data_ptr(), int(ahead),
+                   w.status_ptr(status, dev), L.raw_stream(index))
     if rc:
         L.check(rc, "nsnkv_reserve_pages")
 
@@ -117,7 +113,7 @@ def copy_pages(arrays, src, dst, status=None):
     h, pages, arr = _page_arrays(arrays, dev)
     index = dev.index
     rc = L.call_on(index, L.load().nsnkv_copy_pages, h, pages, len(arrays), arr, src.shape[0], src.data_ptr(),
-                   dst.data_ptr(), _p(status), L.raw_stream(index))
+                   dst.data_ptr(), w.status_ptr(status, dev), L.raw_stream(index))
     if rc:
         L.check(rc, "nsnkv_copy_pages")
 
@@ -148,8 +144,8 @@ def compact_pages(arrays, block_table, page_refs, table_out=None, refs_out=None,
         ws = L.scratch(lib.nsnkv_compact_pages_workspace_bytes(pages), dev, stream)
     rc = L.call_on(index, lib.nsnkv_compact_pages, h, pages, len(arrays), arr, batch, max_blocks,
                    block_table.data_ptr(), block_table.stride(0), table_out.data_ptr(), table_out.stride(0),
-                   page_refs.data_ptr(), refs_out.data_ptr(), live.data_ptr(), ws.data_ptr(), ws.numel(), _p(status),
-                   stream)
+                   page_refs.data_ptr(), refs_out.data_ptr(), live.data_ptr(), ws.data_ptr(), ws.numel(),
+                   w.status_ptr(status, dev), stream)
     if rc:
         L.check(rc, "nsnkv_compact_pages")
     return table_out, refs_out, live

@@ -83,7 +83,7 @@ def prefix_attention(q, records, page_table, n_pages=None, *, bits=3, row_offset
         None if n_pages is None else n_pages.data_ptr(), max_pages,
         None if row_offsets is None else row_offsets.data_ptr(), None if row_index is None else row_index.data_ptr(),
         o_ptr, e_ptr, out.data_ptr(), lse.data_ptr(), ws.data_ptr(), ws.numel(),
-        None if status is None else status.data_ptr(), stream)
+        w.status_ptr(status, dev), stream)
     if rc:
         L.check(rc, "nsnkv_prefix_attn")
     return out, lse

@@ -62,6 +62,15 @@ def _status_to_error(status: int, input_msg: str, meta=True, output_msg="Nonfini
         raise IntegrityError(f"device status {status:#x}")
 
 
+def status_ptr(status, device):
+    """The address of an operator's status word (None: none), which a kernel ORs its bits into."""
+    if status is None:
+        return None
+    require(status.dtype == torch.int32 and status.numel() > 0 and status.device == device,
+            "status: int32 [1] on the operands' device")
+    return status.data_ptr()
+
+
 def code_bytes(bits: int) -> int:
     return BLOCK * DIM * bits // 8
 

@@ -51,7 +51,7 @@ def prompt_attention(q, k, v, cu_seqlens, max_seqlen, *, causal=True, out=None, 
     index = dev.index
     rc = L.call_on(index, L.load().nsnkv_prompt_attn, T, n, int(max_seqlen), hq, h, _TYPES[dt], 1 if causal else 0, qp, qt,
                    qh, kp, kt, kh, vp, vt, vh, cu_seqlens.data_ptr(), out.data_ptr(), lse.data_ptr(),
-                   None if status is None else status.data_ptr(), L.raw_stream(index))
+                   w.status_ptr(status, dev), L.raw_stream(index))
     if rc:
         L.check(rc, "nsnkv_prompt_attn")
     return out, lse

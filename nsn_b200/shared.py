@@ -31,7 +31,8 @@ from .prompt import prompt_attention
 
 class SharedPrefix:
     """Which sequences of a cache share which leading pages, laid out for its step_shared
-    (made by SharedPagedKVCache.share; valid until a fork, free, prefill, import or compaction of it: step_shared refuses it then).
+    (made by SharedPagedKVCache.share; valid until a fork, free, prefill, import or compaction of
+    it, from when on step_shared refuses the plan).
 
     ``own_table`` is a copy of the block table's entries behind the prefixes; step_shared brings it
     up to date when pages were assigned since (by any step, a seal, extend or reserve)."""

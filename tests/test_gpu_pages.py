@@ -220,3 +220,20 @@ def test_free_reports_entries_outside_the_pool():
         s["table"][1] = s["n"][1] = s["tl"][1] = 0
         same(s, d)
         assert int(st) == 128
+
+
+def test_status_elsewhere_is_refused():
+    from nsn_b200 import ContractError
+    from nsn_b200 import pages as P
+    s = state(3, 4, 13)
+    d = {k: dev(v) for k, v in s.items()}
+    rec, one, two = torch.zeros((2, 13, 64), dtype=torch.uint8, device="cuda"), dev(np.int32([0])), dev(np.int32([1]))
+    bad = torch.zeros(1, dtype=torch.int32)
+    for call in (lambda: P.fork_sequences(d["table"], d["n"], d["tl"], d["refs"], d["kt"], d["vt"], one, two, status=bad),
+                 lambda: P.free_sequences(d["table"], d["n"], d["tl"], d["refs"], one, status=bad),
+                 lambda: P.reserve_pages(d["table"], d["n"], d["refs"], status=bad),
+                 lambda: P.copy_pages([rec], one, two, status=bad),
+                 lambda: P.compact_pages([rec], d["table"], d["refs"], status=bad)):
+        with pytest.raises(ContractError):
+            call()
+    same(s, d)

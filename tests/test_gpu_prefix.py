@@ -362,3 +362,12 @@ def test_rows_are_restored_bit_for_bit(bits, dtype):
     known = k.float() * size / math.sqrt(128) > 150  # the other 63 tokens' p are 0
     assert float(known.float().mean()) > 0.9
     assert torch.equal((lse.double() * math.sqrt(128) / size).to(dtype)[known], k[known])
+
+
+def test_status_elsewhere_is_refused():
+    from nsn_b200 import ContractError
+    from nsn_b200.prefix import prefix_attention
+    a, kw, _ = case(1, 2, 3, torch.float16, [2], [3])
+    for bad in (torch.zeros(1, dtype=torch.int32), torch.zeros(1, dtype=torch.int64, device="cuda")):
+        with pytest.raises(ContractError):
+            prefix_attention(*a, status=bad, **kw)

@@ -282,3 +282,12 @@ def test_an_output_that_rounds_past_the_type_is_reported(T):
     out, _ = prompt_attention(q, k, v, cu, T, status=status)
     assert bool(out[-1].isinf().all())  # the case is what it says
     assert int(status) == 8
+
+
+def test_status_elsewhere_is_refused():
+    from nsn_b200 import ContractError
+    from nsn_b200.prompt import prompt_attention
+    q, k, v, cu = make([64], 4, 2, torch.float16)
+    for bad in (torch.zeros(1, dtype=torch.int32), torch.zeros(1, device="cuda")):
+        with pytest.raises(ContractError):
+            prompt_attention(q, k, v, cu, 64, status=bad)

@@ -56,3 +56,16 @@ def test_decode_attention_in_a_graph(capturing, monkeypatch):
     assert kernel.workspace(1 << 9, CPU).data_ptr() == eager.data_ptr()
     capturing["on"] = True
     assert kernel.workspace(1 << 10, CPU).data_ptr() != eager.data_ptr()
+
+
+def test_a_status_word_is_where_the_kernel_can_write_it():
+    """An address of another device's memory is refused on the host, not met by the kernel."""
+    from nsn_b200 import ContractError
+    from nsn_b200.primitives import status_ptr
+    ok = torch.zeros(1, dtype=torch.int32)
+    assert status_ptr(None, ok.device) is None and status_ptr(ok, ok.device) == ok.data_ptr()
+    for bad in (ok.to(torch.int64), ok.float(), ok[:0]):
+        with pytest.raises(ContractError):
+            status_ptr(bad, ok.device)
+    with pytest.raises(ContractError):
+        status_ptr(ok, torch.device("cuda", 0))
