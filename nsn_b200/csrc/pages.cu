@@ -402,7 +402,8 @@ int nsnkv_compact_pages(int h, int64_t pages, int arrays, const nsnkv_page_array
   if (pages > INT32_MAX || batch < 0 || max_blocks < 0 || table_stride < max_blocks || table_out_stride < max_blocks)
     return NSNKV_ERR_ARG;
   if (const int rc = check_arrays(h, pages, arrays, arr)) return rc;
-  if (!page_refs || !refs_out || !live || !workspace || workspace_bytes < nsnkv_compact_pages_workspace_bytes(pages) ||
+  if (!page_refs || !refs_out || !live || !workspace || (reinterpret_cast<uintptr_t>(workspace) & 3) ||
+      workspace_bytes < nsnkv_compact_pages_workspace_bytes(pages) ||
       (batch > 0 && max_blocks > 0 && (!block_table || !table_out)))
     return NSNKV_ERR_ARG;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -142,6 +142,8 @@ def compact_pages(arrays, block_table, page_refs, table_out=None, refs_out=None,
     stream = L.raw_stream(index)
     if ws is None:
         ws = L.scratch(lib.nsnkv_compact_pages_workspace_bytes(pages), dev, stream)
+    else:
+        w.require_workspace(ws, dev)
     rc = L.call_on(index, lib.nsnkv_compact_pages, h, pages, len(arrays), arr, batch, max_blocks,
                    block_table.data_ptr(), block_table.stride(0), table_out.data_ptr(), table_out.stride(0),
                    page_refs.data_ptr(), refs_out.data_ptr(), live.data_ptr(), ws.data_ptr(), ws.numel(),

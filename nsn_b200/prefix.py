@@ -77,6 +77,8 @@ def prefix_attention(q, records, page_table, n_pages=None, *, bits=3, row_offset
     stream = L.raw_stream(index)
     if ws is None:
         ws = L.scratch(lib.nsnkv_prefix_attn_workspace_bytes(rows, groups, hq, rs[0], max_pages), dev, stream)
+    else:
+        w.require_workspace(ws, dev)
     rc = L.call_on(
         index, lib.nsnkv_prefix_attn, rows, groups, int(max_rows or 0), hq, rs[0], bits, _TYPES[dt], q.data_ptr(),
         records.data_ptr(), rs[1], head, page, table.data_ptr(), table.stride(0),

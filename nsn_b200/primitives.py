@@ -71,6 +71,11 @@ def status_ptr(status, device):
     return status.data_ptr()
 
 
+def require_workspace(ws, device):
+    require(ws.dtype == torch.uint8 and ws.is_contiguous() and ws.device == device,
+            "workspace: contiguous uint8 on the operands' device")
+
+
 def code_bytes(bits: int) -> int:
     return BLOCK * DIM * bits // 8
 

@@ -191,3 +191,14 @@ def test_shared_prompt_operators_refuse_on_the_host():
     arr[0].bytes = 64
     assert lib.nsnkv_compact_pages_workspace_bytes(8) >= 100
     assert lib.nsnkv_compact_pages(2, 8, 1, arr, 2, 4, P, 4, P, 4, P, P, P, P, 15, N, N) == _lib.ERR_ARG
+
+
+def test_compaction_workspace_alignment():
+    from nsn_b200 import _lib
+    lib, P, N = _lib.load(), ctypes.c_void_p(16), ctypes.c_void_p(None)
+    arr = (_lib.PageArray * 1)()
+    arr[0].base, arr[0].bytes, arr[0].stride_head, arr[0].stride_page = 16, 64, 640, 64
+    need = lib.nsnkv_compact_pages_workspace_bytes(8)
+    for off in (1, 2, 3):
+        assert lib.nsnkv_compact_pages(2, 8, 1, arr, 2, 4, P, 4, P, 4, P, P, P, ctypes.c_void_p(16 + off), need, N,
+                                       N) == _lib.ERR_ARG

@@ -237,3 +237,14 @@ def test_status_elsewhere_is_refused():
         with pytest.raises(ContractError):
             call()
     same(s, d)
+
+
+def test_workspace_elsewhere_is_refused():
+    from nsn_b200 import ContractError
+    from nsn_b200.pages import compact_pages
+    s = state(3, 4, 13)
+    table, refs, rec = dev(s["table"]), dev(s["refs"]), torch.zeros((2, 13, 64), dtype=torch.uint8, device="cuda")
+    big = torch.empty(1 << 16, dtype=torch.uint8)
+    for bad in (big, big.cuda()[::2]):
+        with pytest.raises(ContractError):
+            compact_pages([rec], table, refs, ws=bad)

@@ -371,3 +371,13 @@ def test_status_elsewhere_is_refused():
     for bad in (torch.zeros(1, dtype=torch.int32), torch.zeros(1, dtype=torch.int64, device="cuda")):
         with pytest.raises(ContractError):
             prefix_attention(*a, status=bad, **kw)
+
+
+def test_workspace_elsewhere_is_refused():
+    from nsn_b200 import ContractError
+    from nsn_b200.prefix import prefix_attention
+    a, kw, _ = case(1, 2, 3, torch.float16, [2], [3])
+    big = torch.empty(1 << 20, dtype=torch.uint8)
+    for bad in (big, big.cuda()[::2]):
+        with pytest.raises(ContractError):
+            prefix_attention(*a, ws=bad, **kw)

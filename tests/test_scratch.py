@@ -69,3 +69,13 @@ def test_a_status_word_is_where_the_kernel_can_write_it():
             status_ptr(bad, ok.device)
     with pytest.raises(ContractError):
         status_ptr(ok, torch.device("cuda", 0))
+
+
+def test_a_workspace_is_where_the_kernel_can_write_it():
+    from nsn_b200 import ContractError
+    from nsn_b200.primitives import require_workspace
+    ok = torch.empty(64, dtype=torch.uint8)
+    require_workspace(ok, ok.device)
+    for bad, device in ((ok.float(), ok.device), (ok[::2], ok.device), (ok, torch.device("cuda", 0))):
+        with pytest.raises(ContractError):
+            require_workspace(bad, device)
