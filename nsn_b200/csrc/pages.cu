@@ -366,6 +366,7 @@ int nsnkv_reserve_pages(int64_t batch, int64_t pages, int32_t *block_table, int6
       table_stride < max_blocks || ahead < 0 || ahead > max_blocks)
     return NSNKV_ERR_ARG;
   if (!block_table || !n_blocks || !page_refs) return NSNKV_ERR_ARG;
+  if (batch * ahead > INT32_MAX) return NSNKV_ERR_TOO_LARGE;  // the kernel counts entries in 32 bits
   reserve_kernel<<<1, kScan, 0, static_cast<cudaStream_t>(stream)>>>(block_table, table_stride, n_blocks, page_refs,
                                                                      pages, static_cast<int32_t>(batch), max_blocks,
                                                                      ahead, status);

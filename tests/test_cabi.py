@@ -202,3 +202,9 @@ def test_compaction_workspace_alignment():
     for off in (1, 2, 3):
         assert lib.nsnkv_compact_pages(2, 8, 1, arr, 2, 4, P, 4, P, 4, P, P, P, ctypes.c_void_p(16 + off), need, N,
                                        N) == _lib.ERR_ARG
+
+
+def test_reserve_refuses_more_entries_than_it_can_count():
+    from nsn_b200 import _lib
+    lib, P, N = _lib.load(), ctypes.c_void_p(16), ctypes.c_void_p(None)
+    assert lib.nsnkv_reserve_pages(1 << 20, 8, P, 4096, 4096, P, P, 2048, N, N) == _lib.ERR_TOO_LARGE
