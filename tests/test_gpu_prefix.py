@@ -381,3 +381,47 @@ def test_workspace_elsewhere_is_refused():
     for bad in (big, big.cuda()[::2]):
         with pytest.raises(ContractError):
             prefix_attention(*a, ws=bad, **kw)
+
+
+@pytest.mark.parametrize("growth", ["level", "rising", "spike", "falling"])
+@pytest.mark.parametrize("bits,dtype,counts,rows,wide,most", [
+    (3, torch.float16, [11], [3], 888, None),          # one row tile, both teams on it: three blocks each
+    (5, torch.float16, [13], [3], 888, None),
+    (3, torch.bfloat16, [11], [40], 888, None),        # two row tiles, the second in part
+    (3, torch.float16, [9, 14], [20, 70], 888, None),
+    (5, torch.bfloat16, [17], [300], 180, 1),          # a CTA takes several pairs of row tiles in turn
+    (3, torch.float16, [17], [300], 180, 1)])
+def test_many_blocks_per_cta(bits, dtype, counts, rows, wide, most, growth):
+    """Chunks of several blocks: P.V accumulated, both S buffers used again, the maximum in use
+    raised with O rescaled (K of later blocks larger), or never raised."""
+    from nsn_b200 import _lib as L
+    from nsn_b200.prefix import prefix_attention
+    g = torch.Generator(device="cuda").manual_seed(7)
+    pages, G = sum(counts) + 2, 4
+    rec, kp, vp = pool(1, pages, bits, 5)
+    order = torch.randperm(pages, generator=g, device="cuda").tolist()
+    table, at = [], 0
+    for n in counts:
+        for i, p in enumerate(order[at:at + n]):
+            kp["alpha"][:, p] *= {"level": 1.0, "rising": 1.7 ** (i % 6), "spike": 12.0 if i % 6 == 3 else 1.0,
+                                  "falling": 1.7 ** (5 - i % 6)}[growth]
+        table.append(order[at:at + n])
+        at += n
+    total = sum(rows)
+    q = torch.randn((total, G, 128), generator=g, device="cuda").to(dtype)
+    o_part = torch.randn((total, G, 128), generator=g, device="cuda")
+    lse_part = 5 + torch.randn((total, G), generator=g, device="cuda")
+    index = torch.randperm(total, generator=g, device="cuda").tolist()
+    offsets = [sum(rows[:i]) for i in range(len(rows) + 1)]
+    t = torch.zeros((len(counts), wide), dtype=torch.int32, device="cuda")
+    dev = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    for i, r in enumerate(table):
+        t[i, :len(r)] = dev(r)
+    chunks = L.load().nsnkv_prefix_attn_workspace_bytes(total, len(counts), G, 1, wide) // (total * G * 129 * 4)
+    assert -(-wide // chunks) >= 4  # blocks per CTA
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    got = prefix_attention(q, rec, t, dev(counts), bits=bits, row_offsets=dev(offsets), row_index=dev(index),
+                           max_rows=most or max(rows), o_part=o_part, lse_part=lse_part, status=status)
+    check(got, reference(q, rows_of(kp, bits, dtype), rows_of(vp, bits, dtype), table, counts, offsets, index, o_part,
+                         lse_part))
+    assert int(status) == 0

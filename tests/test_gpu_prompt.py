@@ -291,3 +291,30 @@ def test_status_elsewhere_is_refused():
     for bad in (torch.zeros(1, dtype=torch.int32), torch.zeros(1, device="cuda")):
         with pytest.raises(ContractError):
             prompt_attention(q, k, v, cu, 64, status=bad)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_several_long_items_per_cta(causal):
+    """More pairs of row tiles than SMs, of several K / V tiles each: S of the next item is
+    issued while an item ends."""
+    from nsn_b200.prompt import prompt_attention
+    lens = [1500, 200, 700, 1100]
+    q, k, v, cu = make(lens, 40, 8, torch.bfloat16, fused=True)
+    out, lse = prompt_attention(q, k, v, cu, 1500, causal=causal)
+    check(out, lse, reference(q, k, v, lens, causal))
+
+
+def test_unseen_values_in_later_items():
+    """Non-finite V in the shorter sequences, whose items are a CTA's second and later ones."""
+    from nsn_b200.prompt import prompt_attention
+    lens = [1500, 600, 450]
+    q, k, v, cu = make(lens, 40, 8, torch.float16)
+    ref = reference(q, k, v, lens)
+    bad = torch.zeros(sum(lens), dtype=torch.bool, device="cuda")
+    for first, last in ((1500 + 580, 2100), (2100 + 449, 2550)):
+        v[first:last] = math.nan
+        bad[first:last] = True
+    out, lse = prompt_attention(q, k, v, cu, 1500)
+    assert bool(out[bad].isnan().all())
+    check(out, lse, ref, ~bad)
+    assert bool(((lse.double() - ref[1]).abs() <= ref[3])[bad].all())  # lse does not look at V
