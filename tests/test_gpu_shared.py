@@ -317,3 +317,41 @@ def test_a_full_sequence_refuses_the_shared_step():
         assert shared.host_blocks.tolist() == [3, 3] and shared.host_tail.tolist() == [63, 63]
         refs_hold(shared)
     shared.check()
+
+
+@pytest.mark.parametrize("prompt,new", [(200, 50), (128, 1), (64 * 3 + 63, 130)])
+def test_a_new_turn_after_a_cached_prompt(prompt, new):
+    """The new tokens' queries over sealed blocks, cached tail and new tokens: prompt attention over
+    tail and new tokens (the tail's rows are dropped), merged with the sealed blocks.
+
+    Bound: the output's rounding u |o|, the probabilities' u sum p |v| in both parts, the own
+    part's rounding, at most u sum p |v| again, and scores as in tests/test_gpu_prompt.py."""
+    import test_gpu_prefix as R
+    from nsn_b200.prefix import prefix_attention
+    from nsn_b200.prompt import prompt_attention
+    from nsn_b200.shared import SharedPagedKVCache
+    h, hq, u = 2, 8, 2.0 ** -11
+    c = SharedPagedKVCache(1, h, 6, 12, hq=hq)
+    c.prefill(0, *rows(prompt, h, 3))
+    k, v = rows(new, h, 4)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    q = torch.randn((new, hq, 128), generator=g, device="cuda").half()
+    n, t = int(c.host_blocks[0]), int(c.host_tail[0])
+    own_k, own_v = (torch.cat([tail[0, :, :t], x], 1).transpose(0, 1) for tail, x in ((c.k_tail, k), (c.v_tail, v)))
+    own_q = torch.cat([q.new_zeros((t, hq, 128)), q])
+    cu = torch.tensor([0, t + new], dtype=torch.int32, device="cuda")
+    o, e = prompt_attention(own_q, own_k, own_v, cu, t + new)
+    out, _ = prefix_attention(q, c.records, c.block_table[:1, :n], o_part=o[t:].float(), lse_part=e[t:].contiguous())
+    pages = c.block_table[0, :n].long()
+    sealed = [R.rows_of({a: b[:, pages] if torch.is_tensor(b) else b for a, b in p.items()}, 3, torch.float16)
+              for p in (c.k_pool, c.v_pool)]
+    kk, vv = (torch.cat([s.reshape(h, 64 * n, 128), x.transpose(0, 1)], 1).double() for s, x in zip(sealed,
+                                                                                                    (own_k, own_v)))
+    seen = torch.arange(prompt + new, device="cuda")[None] <= prompt + torch.arange(new, device="cuda")[:, None]
+    for j in range(hq):
+        x = q[:, j].double() @ kk[j // 4].T / 128 ** 0.5
+        dx = 2.0 ** -20 * (1 + (q[:, j].double().abs() @ kk[j // 4].abs().T).amax(1, keepdim=True) / 128 ** 0.5)
+        p = torch.softmax(x.masked_fill(~seen, -float("inf")), 1)
+        want, big = p @ vv[j // 4], p @ vv[j // 4].abs()
+        tol = u * (want.abs() + 2 * big) * 1.01 + 5 * dx * big + (prompt + new) * 2.0 ** -25 * vv.abs().amax()
+        assert bool(((out[:, j].double() - want).abs() <= tol).all()), j
