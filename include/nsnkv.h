@@ -496,8 +496,8 @@ int nsnkv_k1c_scores(int recipe, int64_t batch, int n_q, int n_kv, int64_t token
  *                scores (may be NULL)
  * Scores use scale 1/sqrt(128); softmax statistics and accumulation are fp32, the
  * probabilities are rounded to dtype for the product with V.  A token that a row does not
- * see does not reach it, NaN and infinities included.  NSNKV_ST_OUTPUT_NONFINITE when an
- * output is not finite.
+ * see does not reach it, NaN and infinities included; a row with a NaN score has a NaN output
+ * and log-sum-exp.  NSNKV_ST_OUTPUT_NONFINITE when an output, rounded to dtype, is not finite.
  */
 int nsnkv_prompt_attn(int64_t tokens, int32_t seqs, int64_t longest, int hq, int h, int dtype, int causal,
                       const void *q, int64_t q_tok, int64_t q_head, const void *k, int64_t k_tok, int64_t k_head,
@@ -524,7 +524,7 @@ int nsnkv_prompt_attn(int64_t tokens, int32_t seqs, int64_t longest, int hq, int
  *   o_part, lse_part  fp32 [rows][hq][128] and [rows][hq]: normalised output and natural
  *                log-sum-exp over each row's own tokens (-inf: none); both NULL: no merge
  *   out, lse     as for nsnkv_prompt_attn, over prefix and own tokens; a row that sees
- *                nothing gets zeros and -inf
+ *                nothing gets zeros and -inf, a row with a NaN score or lse_part NaN in both
  *   workspace    nsnkv_prefix_attn_workspace_bytes() bytes, 16-byte aligned, any contents;
  *                calls that may run at the same time need separate ones
  * Status: NSNKV_ST_INPUT_NONFINITE (q or a record's metadata), NSNKV_ST_OUTPUT_NONFINITE,
@@ -551,7 +551,7 @@ int nsnkv_prefix_attn(int64_t rows, int32_t groups, int64_t max_rows, int hq, in
  * nsnkv_fork_sequences: sequence dst[i] becomes a copy of sequence src[i], i < count: it drops
  * its pages, shares src's sealed pages (reserved ones are not shared), and copies src's
  * counters and tail rows (16-bit tails, strides in rows of 128 elements).  The dst are
- * distinct and none of them is a src.
+ * distinct and none of them is a src.  A source entry outside [0, pages) is 0 in dst.
  * nsnkv_free_sequences: sequences drop their pages and are empty.
  * nsnkv_reserve_pages: every sequence gets pages for its next `ahead` blocks where its entries
  * n_blocks[b] .. n_blocks[b] + ahead - 1 name none; in (sequence, entry) order they take the

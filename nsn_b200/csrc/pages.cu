@@ -114,7 +114,8 @@ __device__ __forceinline__ int block_scan(int x, int &sum) {
 }
 
 // Table entries n_blocks[b] .. n_blocks[b] + ahead - 1 that name no page get free pages: the
-// entries in (sequence, entry) order take the free pages in ascending order.
+// entries in (sequence, entry) order take the free pages in ascending order.  One CTA: 12 us a
+// call for 64 sequences, most of it the launch and the call.
 __global__ void __launch_bounds__(kScan) reserve_kernel(int32_t *table, int64_t table_stride, const int32_t *n_blocks,
                                                         int32_t *refs, int64_t pages, int32_t batch, int32_t max_blocks,
                                                         int32_t ahead, int32_t *status) {
@@ -248,8 +249,8 @@ struct MoveArgs {
 // Work item (move i, head j): the page's bytes of every array in 16-byte pieces, kPieces per
 // thread and round, all loaded before the first is stored (a page is at most a few KB: one or
 // two rounds).  The next item's page numbers are read while an item is copied.  4800 pages of
-// eight heads, INT3 (610 MB read and written): 136 us with the plan, 4.5 TB/s; with the loads
-// and stores of a piece in turn it was 192 us.
+// eight heads, INT3 (610 MB read and written): 138 us with the plan, 4.4 TB/s (timed apart: move
+// 109 us, plan 20 us); with the loads and stores of a piece in turn it was 192 us.
 constexpr int kMoveThreads = 128, kPieces = 4;
 __global__ void __launch_bounds__(kMoveThreads) move_kernel(const MoveArgs a) {
   const int tid = threadIdx.x;

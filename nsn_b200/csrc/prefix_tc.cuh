@@ -19,9 +19,10 @@
 // alpha 2^32 takes the factor back in the product (alpha is at most 65504 / 1e-12).  a and b are
 // laid out once per block and channel.
 //
-// Measured: 64 rows over 8192 INT3 tokens, GQA 32:8: 35.4 us with the merge (eight blocks per CTA at
+// Measured: 64 rows over 8192 INT3 tokens, GQA 32:8: 35.6 us with the merge (eight blocks per CTA at
 // 2400 cycles between a start of 9 k cycles and 8 k of writing partial rows); 8 rows over 131008
-// INT5 tokens, GQA 64:8: 156 us (1.24 TB/s of records, 0.5 instructions per cycle and scheduler).
+// INT5 tokens, GQA 64:8: 156 us (1.24 TB/s of records, 0.52 instructions per cycle and scheduler,
+// 4580 a block).  640 threads leave 96 registers each, and some 80 bytes a thread are spilled.
 // Blocks of 64 tokens, not 128, leave TMEM for two buffers of S per team and shared memory for
 // four restored blocks.
 #pragma once

@@ -14,9 +14,9 @@
 // tensor core adds P.V to O, P read from TMEM.  While one row tile is in its softmax the
 // tensor core works on the other.
 //
-// Measured: 16384 tokens, GQA 32:8, fp16: 1.79 ms in a short run (1230 TFLOP/s, 0.75 of the
+// Measured: 16384 tokens, GQA 32:8, fp16: 1.76 ms in a short run (1250 TFLOP/s, 0.76 of the
 // library GEMM's burst rate), 2.12 ms under sustained load, where the power limit holds the clock;
-// 4 x 2048 tokens, 16 heads: 98 us.  What bounds it is the chain S -> softmax -> P.V of one row
+// 4 x 2048 tokens, 16 heads: 99 us.  What bounds it is the chain S -> softmax -> P.V of one row
 // tile with one warp per scheduler (about 2450 of 3150 cycles per K / V tile are softmax); the
 // tensor pipe is busy 43% to 50% of the time.  Tiles are 128 tokens because Q.K^T with both operands in shared
 // memory reads 128 bytes a cycle at N = 128, all that shared memory gives, and more below.
